@@ -160,7 +160,7 @@ def _handle(case, pages, blocks, device=0):
     heads, kv, hs, page = case.get("heads", 1), case.get("kv_heads", 1), case.get("head_size", 64), case["page"]
     strides = (page * kv * hs, kv * hs, hs) if case.get("layout") != "head" else (page * kv * hs, hs, page * hs)
     return pk_b200.KvPaged(heads, kv, hs, pk_b200.F16 if case.get("cache") == "f16" else pk_b200.F32, page, pages,
-                           case["n"], blocks, strides=strides, device=device)
+                           case["n"] if case["op"] != "append" else 1, blocks, strides=strides, device=device)
 
 
 def prepare(case, seed):
