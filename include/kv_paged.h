@@ -1,0 +1,147 @@
+/*
+ * kv_paged.h - a paged key-value cache on the device: block tables and slot
+ * maps from the requests' lengths, the append of a step's keys and values
+ * with their rotary positions, and the attention of single new tokens over
+ * the pages. engine_batch_open_paged (engine_ext.h) decodes through these
+ * calls; they have no counterpart in the reference, whose run state keeps one
+ * contiguous cache per sequence.
+ *
+ * The cache of one layer is two pools (keys, values) of n_pages pages of
+ * page_tokens tokens. Token t of request i lies in page
+ * table[i * max_blocks + t / page_tokens] at place t % page_tokens; the slot
+ * of a token is page * page_tokens + place. Several layers share one block
+ * table: each has its own pools of the same shape.
+ *
+ * A step is three calls on one stream:
+ *   kv_paged_map      len, start, end -> pages, rows (request, position, slot)
+ *   kv_paged_append   per layer: q, k, v -> q turned, k and v in their slots
+ *   kv_paged_attend   per layer: q -> out
+ * Rows behind the step's last row hold -1 and are passed over by every call,
+ * so a step captured in a CUDA graph for max_rows rows serves any smaller one.
+ *
+ * Calls are asynchronous on `stream` (a cudaStream_t of the handle's device,
+ * NULL for its default stream); pointers are device pointers on that device
+ * unless noted. The current device may be another one: it is left as it was.
+ * Calls return 1, or 0 on bad arguments or a failed launch (nothing is
+ * launched on bad arguments; kv_paged_last_error has the message). All
+ * of them may be captured into a CUDA graph.
+ *
+ * A handle owns the scratch of its calls. Calls of one handle that may
+ * overlap in time (two streams, two graphs replayed side by side) race on
+ * it: give each its own handle. Handles may share pools and tables.
+ */
+#ifndef KV_PAGED_H
+#define KV_PAGED_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define KV_PAGED_MAX_REQUESTS 4096
+
+typedef struct {
+    int n_heads;         /* query heads, a multiple of n_kv_heads */
+    int n_kv_heads;      /* query head h reads KV head h / (n_heads / n_kv_heads) */
+    int head_size;       /* a multiple of 8, 8 .. 256 */
+    uint32_t type;       /* GGML type id of the pools' entries: 0 F32 or 1 F16 */
+    int page_tokens;     /* tokens of a page, any number >= 1 */
+    int n_pages;         /* pages of a pool; n_pages * page_tokens < 2^31 */
+    int max_requests;    /* rows of the block table, 1 .. KV_PAGED_MAX_REQUESTS */
+    int max_blocks;      /* entries of a row of the block table */
+    /* Entries from a page, token or KV head to the next, multiples of 16
+     * bytes; all 0: [page][token][KV head][channel] without gaps. Channels
+     * are adjacent. */
+    uint64_t page_stride, token_stride, head_stride;
+} KvPagedShape;
+
+typedef struct KvPaged KvPaged;
+
+/* A handle for calls on `device`. NULL on failure with a message in error
+ * (may be NULL). device -1 makes a handle that checks the arguments of calls
+ * and launches nothing (good ones return 0 with "The handle has no device."). */
+KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *error, size_t error_capacity);
+
+/* Safe on NULL. Waits for the device (it frees device memory). */
+void kv_paged_close(KvPaged *kv);
+
+/* Why the last call of this handle returned 0 ("" if none did). */
+const char *kv_paged_last_error(const KvPaged *kv);
+
+/* What the device found wrong since the last query, as bits; read and
+ * cleared (waits for the device; not during a capture). -1: unreadable. */
+#define KV_PAGED_NO_PAGES 1    /* map: more pages needed than free: nothing changed, no rows */
+#define KV_PAGED_NO_ROWS 2     /* map: more than max_rows rows: nothing changed, no rows */
+#define KV_PAGED_BAD_LENGTH 4  /* map: not 0 <= start <= len, start <= end, both ends within the table,
+                                  or n_free outside 0 .. n_pages: nothing changed, no rows */
+#define KV_PAGED_BAD_PAGE 8    /* a page outside the pool was met: map gives such rows slot -1, attend
+                                  leaves its tokens out */
+#define KV_PAGED_BAD_ROW 16    /* append: a slot past the pool or a position past the rotary table (row
+                                  passed over); attend: a request past the table (row passed over) or a
+                                  position past its row (its tokens end at the row's last) */
+int kv_paged_error(KvPaged *kv);
+
+/*
+ * Pages and rows of a step. Request i < n holds the pages of len[i] tokens;
+ * its rows of this step are the positions start[i] .. end[i] - 1, and it
+ * holds the pages of end[i] tokens afterwards. start[i] < len[i] takes
+ * tokens back first (a rejected draft); end[i] = start[i] means no rows;
+ * start = end = 0 gives a request's pages back. 0 <= start <= len, start <= end.
+ *
+ * free_pages (room for n_pages) is a stack of free page numbers, *n_free of
+ * them. The pages of blocks behind end[i] are pushed first, in the order of
+ * requests and blocks (table entries of pages given back stay as they
+ * are), then the pages of new blocks are popped from the top in that order,
+ * into the table. *n_free_out receives the new count; it may be n_free
+ * itself, and where it is not, the same call can be made again from the same
+ * state. No page is pushed or popped unless all of the step's can be.
+ *
+ * row0 (n + 1 numbers) receives each request's first row and the row count;
+ * row_request, row_pos and row_slot (max_rows each) the rows, request after
+ * request, then -1 to max_rows.
+ */
+int kv_paged_map(KvPaged *kv, const int *len, const int *start, const int *end, int n, int *table,
+                 int *free_pages, const int *n_free, int *n_free_out, int max_rows, int *row_request,
+                 int *row_pos, int *row_slot, int *row0, void *stream);
+
+/*
+ * Rows r < n with row_slot[r] >= 0: q_out[r] = q[r] turned by the rotary
+ * positions of row_pos[r], and k[r] (turned) and v[r] into slot row_slot[r]
+ * of the pools, rounded to nearest even in an F16 pool. Channels 2i, 2i + 1
+ * < rope_dim of every head turn by the pair (cos, sin) at
+ * rope_cs[pos * rope_dim + 2i], as in reference src/gguf_forward.c:50-66;
+ * further channels stay. rope_dim 0 (rope_cs NULL) turns nothing; rope_len is the
+ * number of positions in rope_cs. Slots of one call are distinct.
+ *
+ * q and q_out: rows of n_heads * head_size floats; q_out may be q, and q and
+ * q_out may both be NULL. k and v: rows of n_kv_heads * head_size floats.
+ * q_stride and kv_stride: floats from a row of q, and of k and v, to the
+ * next (0: without gaps; multiples of 4). q_out has no gaps unless it is q.
+ * All but row_pos and row_slot on 16 bytes (rope_cs on 8).
+ */
+int kv_paged_append(KvPaged *kv, const float *q, const float *k, const float *v, const int *row_pos,
+                    const int *row_slot, int n, float *q_out, void *k_pool, void *v_pool, const float *rope_cs,
+                    int rope_dim, int rope_len, uint64_t q_stride, uint64_t kv_stride, void *stream);
+
+/*
+ * Attention of rows r < n, each a single token of request row_request[r] at
+ * position row_pos[r], over that request's tokens 0 .. row_pos[r]:
+ * out[r][h] = sum_t p_t v_t with p = softmax(scale * q[r][h] . k_t), in
+ * float. row_pos -1 gives zeros; a row with row_request < 0 is passed over
+ * and its output left as it was. Entries of the pools behind a row's
+ * position are never used, whatever they hold. table has n_requests
+ * (<= max_requests) rows. q and out: rows of n_heads * head_size floats on
+ * 16 bytes, q_stride as in kv_paged_append; out must not overlap q. Results do
+ * not depend on timing: the same inputs give the same bits.
+ */
+int kv_paged_attend(KvPaged *kv, const float *q, const void *k_pool, const void *v_pool, const int *table,
+                    int n_requests, const int *row_request, const int *row_pos, int n, float scale, float *out,
+                    uint64_t q_stride, void *stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif

@@ -1,4 +1,5 @@
-"""ctypes binding of libpocketllm_b200.so (engine.h, engine_ext.h, gguf_cuda.h).
+"""ctypes binding of libpocketllm_b200.so (engine.h, engine_ext.h, gguf_cuda.h,
+kv_paged.h).
 
 This is how Python callers (the tests, bench.py) reach the C ABI, in the
 same style as the reference's ctypes package (python/pocketllm/__init__.py).
@@ -33,6 +34,12 @@ EXPORTS = [
     "gguf_cuda_matvec_error", "gguf_cuda_matvec_noalloc_error",
     "gguf_cuda_matmul", "gguf_cuda_matmul_plan", "gguf_cuda_matmul_error",
     "tokenizer_free",
+]
+
+# ... and the symbols of include/kv_paged.h.
+KV_PAGED_EXPORTS = [
+    "kv_paged_open", "kv_paged_close", "kv_paged_last_error", "kv_paged_error", "kv_paged_map", "kv_paged_append",
+    "kv_paged_attend",
 ]
 
 
@@ -79,6 +86,12 @@ class GGUFWeight(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("data", _P), ("type", ctypes.c_uint32),
                 ("cols", ctypes.c_uint64), ("rows", ctypes.c_uint64),
                 ("row_bytes", ctypes.c_uint64), ("byte_size", ctypes.c_uint64)]
+
+
+class KvPagedShape(ctypes.Structure):  # include/kv_paged.h
+    _fields_ = [(n, ctypes.c_int) for n in ("n_heads", "n_kv_heads", "head_size")] + [("type", ctypes.c_uint32)] + \
+               [(n, ctypes.c_int) for n in ("page_tokens", "n_pages", "max_requests", "max_blocks")] + \
+               [(n, ctypes.c_uint64) for n in ("page_stride", "token_stride", "head_stride")]
 
 
 _lib = None
@@ -166,6 +179,21 @@ def lib(path=LIB_PATH):
                                         ctypes.POINTER(ctypes.c_int)]
     L.gguf_cuda_matmul_error.restype = ctypes.c_int
     L.gguf_cuda_matmul_error.argtypes = []
+    I, U = ctypes.c_int, ctypes.c_uint64
+    L.kv_paged_open.restype = _P
+    L.kv_paged_open.argtypes = [ctypes.POINTER(KvPagedShape), I, ctypes.c_char_p, ctypes.c_size_t]
+    L.kv_paged_close.restype = None
+    L.kv_paged_close.argtypes = [_P]
+    L.kv_paged_last_error.restype = ctypes.c_char_p
+    L.kv_paged_last_error.argtypes = [_P]
+    L.kv_paged_error.restype = I
+    L.kv_paged_error.argtypes = [_P]
+    L.kv_paged_map.restype = I
+    L.kv_paged_map.argtypes = [_P, _P, _P, _P, I, _P, _P, _P, _P, I, _P, _P, _P, _P, _P]
+    L.kv_paged_append.restype = I
+    L.kv_paged_append.argtypes = [_P, _P, _P, _P, _P, _P, I, _P, _P, _P, _P, I, I, U, U, _P]
+    L.kv_paged_attend.restype = I
+    L.kv_paged_attend.argtypes = [_P, _P, _P, _P, _P, I, _P, _P, I, ctypes.c_float, _P, U, _P]
     _lib = L
     return L
 
@@ -319,6 +347,58 @@ class Engine:
     def close(self):
         if self.h:
             lib().engine_close(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KvPaged:
+    """One kv_paged_open() handle: a paged KV cache's calls (include/kv_paged.h).
+    Pools, tables and rows are the caller's device memory, given as addresses;
+    refused calls raise RuntimeError."""
+
+    def __init__(self, n_heads, n_kv_heads, head_size, qtype, page_tokens, n_pages, max_requests, max_blocks,
+                 strides=(0, 0, 0), device=0):
+        L = lib()
+        shape = KvPagedShape(n_heads, n_kv_heads, head_size, qtype, page_tokens, n_pages, max_requests, max_blocks,
+                             *strides)
+        err = ctypes.create_string_buffer(256)
+        self.h = L.kv_paged_open(ctypes.byref(shape), device, err, 256)
+        if not self.h:
+            raise RuntimeError("kv_paged_open failed: " + err.value.decode())
+        self._map, self._append, self._attend = L.kv_paged_map, L.kv_paged_append, L.kv_paged_attend
+
+    def map(self, len_ptr, start, end, n, table, free_pages, n_free, n_free_out, max_rows, row_request, row_pos,
+            row_slot, row0, stream=0):
+        if self._map(self.h, len_ptr, start, end, n, table, free_pages, n_free, n_free_out, max_rows, row_request,
+                     row_pos, row_slot, row0, stream) != 1:
+            raise RuntimeError("kv_paged_map failed: " + self.last_error())
+
+    def append(self, q, k, v, row_pos, row_slot, n, q_out, k_pool, v_pool, rope_cs=0, rope_dim=0, rope_len=0,
+               q_stride=0, kv_stride=0, stream=0):
+        if self._append(self.h, q, k, v, row_pos, row_slot, n, q_out, k_pool, v_pool, rope_cs, rope_dim, rope_len,
+                        q_stride, kv_stride, stream) != 1:
+            raise RuntimeError("kv_paged_append failed: " + self.last_error())
+
+    def attend(self, q, k_pool, v_pool, table, n_requests, row_request, row_pos, n, scale, out, q_stride=0, stream=0):
+        if self._attend(self.h, q, k_pool, v_pool, table, n_requests, row_request, row_pos, n, scale, out, q_stride,
+                        stream) != 1:
+            raise RuntimeError("kv_paged_attend failed: " + self.last_error())
+
+    def error(self):
+        """kv_paged_error: what the device found wrong since the last query, as bits (0: nothing)."""
+        return lib().kv_paged_error(self.h)
+
+    def last_error(self):
+        return lib().kv_paged_last_error(self.h).decode()
+
+    def close(self):
+        if self.h:
+            lib().kv_paged_close(self.h)
             self.h = None
 
     def __del__(self):
