@@ -131,7 +131,8 @@ int kv_paged_append(KvPaged *kv, const float *q, const float *k, const float *v,
  * out[r][h] = sum_t p_t v_t with p = softmax(scale * q[r][h] . k_t), in
  * float. row_pos -1 gives zeros; a row with row_request < 0 is passed over
  * and its output left as it was. Entries of the pools behind a row's
- * position are never used, whatever they hold. table has n_requests
+ * position are never used, whatever they hold; visible entries of an F32 pool
+ * are below 2^127 in size. table has n_requests
  * (<= max_requests) rows. q and out: rows of n_heads * head_size floats on
  * 16 bytes, q_stride as in kv_paged_append; out must not overlap q. Results do
  * not depend on timing: the same inputs give the same bits.

@@ -293,95 +293,594 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
 // attend                                                             //
 // ------------------------------------------------------------------ //
 
-constexpr int ATT_WARPS = 4;
+// A work item is one row's KV head with up to 8 of its query heads. The 8
+// heads are the upper half of a 16-row matrix operand, what they lose in
+// rounding to the operand's 11 bits is the lower half (rows 8..15), and the
+// accumulator's two halves, which each thread holds side by side, are added:
+// q (and p, the same way) counts with 22 bits at no extra product. A float
+// cache's entries are split likewise into two tf32 parts, two products each;
+// a half cache's are exact. With 16 rows at most, a tcgen05 tile (64 rows at
+// least, operands through shared memory and accumulators through tensor
+// memory) would do four times the work for the same bytes: the warp-level
+// mma takes its operands straight from the registers that the softmax leaves
+// them in.
+//
+// Every warp of a CTA runs a ring of its own: STAGES tiles of TILE tokens
+// (keys and values, about 9 KB) are in flight by 16-byte async copies, with
+// the page numbers of the tile after them; a warp waits for no other before
+// an item's end. Tokens that a row may not see are zero-filled, never read.
+constexpr int ATT_WARPS = 4, ATT_STAGES = 3, ATT_HEADS = 8;
+
+template <typename KV, int HSP>
+struct Geo {
+    static constexpr bool HALF = sizeof(KV) == 2;
+    static constexpr int TILE = HALF ? (HSP == 64 ? 32 : 16) : (HSP == 64 ? 16 : 8);  // tokens
+    static constexpr int CHUNK = ATT_WARPS * TILE;   // tokens: the unit in which work is shared out
+    static constexpr int ROW = HSP * (int)sizeof(KV) + 16;  // bytes; 16 past a multiple of 128: no bank conflicts
+    static constexpr int STAGE = 2 * TILE * ROW;
+    static constexpr int RING = ATT_STAGES * STAGE;
+    static constexpr int SEGS = HSP * (int)sizeof(KV) / 16;  // 16-byte pieces of a token's head
+    static constexpr int QFRAG = (HALF ? HSP / 16 : HSP / 8) * 512;
+    static constexpr int SMEM = ATT_WARPS * RING + QFRAG;
+    static constexpr int OROW = HSP + 8;  // floats from a head to the next where warps leave their sums
+    static_assert(ATT_HEADS * OROW * 4 <= STAGE, "a warp's sums fit a stage");
+};
 
 struct AttendArgs {
     const float *q;
     const void *k_pool, *v_pool;
     const int *table, *row_request, *row_pos;
     int n, n_requests, heads, kv_heads, hs;
+    int groups, group_heads;  // a KV head's items, and the query heads of each
     float scale;
     float *out;
     uint64_t q_stride;
     Cache c;
+    float *part;        // [2 * grid][ATT_HEADS][HSP + 2]: sums, then maximum and weight
+    unsigned *arrived;  // [grid]: parts of the item that begins in CTA b and ends in another; wraps to 0 by itself
     int *err;
 };
 
-__device__ __forceinline__ float kv_get(const float *p)
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr)
 {
-    return *p;
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
 }
-__device__ __forceinline__ float kv_get(const __half *p)
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr)
 {
-    return __half2float(*p);
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// x = hi + lo, hi rounded to tf32's 11 bits: lo is at most half of hi's last
+// place, 12 bits of which the product reads 11 (the upper 19 bits of a word),
+// so at most 2^-23 of x is lost. (Cutting hi off instead of rounding it
+// leaves 13 bits in lo and loses up to 2^-21.)
+__device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
+{
+    hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+// (x, y) = hi + lo, each a pair of halves.
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo)
+{
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
-// One CTA per (row, query head). Warp w takes tokens w, w + ATT_WARPS, ...:
-// its lanes share the channels of a token's key, and keep a running maximum
-// m, sum l and weighted values o; the warps' are joined at the end.
-template <typename KV>
+// Row r's visible tokens, -1 for a row that is passed over.
+__device__ __forceinline__ int row_tokens(const AttendArgs &a, int r, int &fault)
+{
+    const int req = a.row_request[r], last = a.row_pos[r];
+    if (req < 0) return -1;
+    if (req >= a.n_requests) {
+        fault = KV_PAGED_BAD_ROW;
+        return -1;
+    }
+    const int cap = a.c.max_blocks * (int)a.c.page.d;
+    if (last < -1 || last >= cap) {
+        fault = KV_PAGED_BAD_ROW;
+        return last < 0 ? 0 : cap;
+    }
+    return last + 1;
+}
+
+__host__ __device__ __forceinline__ int chunks_of(int tokens, int chunk)
+{
+    return tokens < 0 ? 0 : tokens == 0 ? 1 : (tokens - 1) / chunk + 1;
+}
+
+// A place in a CTA's share of the work: chunk `c` of item `it` of row r.
+struct Place {
+    int r, it, tokens, c;
+    long long left;  // chunks of the CTA's share from here on
+
+    // chunks of this item in the share
+    __device__ __forceinline__ int span(int chunk) const
+    {
+        const int k = chunks_of(tokens, chunk) - c;
+        return left < k ? (int)left : k;
+    }
+    // on to the next item; the share has one more when left > 0
+    __device__ __forceinline__ void next(const AttendArgs &a, int chunk, int items)
+    {
+        left -= span(chunk);
+        c = 0;
+        if (++it < items || left <= 0) return;
+        it = 0;
+        int unused;
+        do {
+            if (++r >= a.n) {  // not while the rows stay as they were counted
+                left = 0;
+                return;
+            }
+            tokens = row_tokens(a, r, unused);
+        } while (tokens < 0);
+    }
+};
+
+template <typename KV, int HSP>
 __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs a)
 {
-    __shared__ float part[ATT_WARPS][256 + 2];
-    const int r = blockIdx.y, h = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int req = a.row_request[r];
-    if (req < 0) return;
-    int last = a.row_pos[r];
-    const int cap = min((long long)a.c.max_blocks * a.c.page.d, 0x7FFFFFFFll);
-    if (req >= a.n_requests) {
-        if (threadIdx.x == 0) atomicOr(a.err, KV_PAGED_BAD_ROW);
-        return;
-    }
-    if (last < -1 || last >= cap) {
-        if (threadIdx.x == 0) atomicOr(a.err, KV_PAGED_BAD_ROW);
-        last = last < 0 ? -1 : cap - 1;
-    }
-    const float *q = a.q + r * a.q_stride + (size_t)h * a.hs;
-    const size_t head = (size_t)(h / (a.heads / a.kv_heads)) * a.c.head_stride;
-    float qv[8], o[8], m = -INFINITY, l = 0.0f;
+    using G = Geo<KV, HSP>;
+    constexpr int TILE = G::TILE, CHUNK = G::CHUNK, W = ATT_WARPS, NT = TILE / 8, DT = HSP / 8;
+    extern __shared__ __align__(16) uint8_t smem[];  // rings, then q
+    __shared__ float row_unit[ATT_HEADS];            // score = product * row_unit
+    __shared__ float wm[W][ATT_HEADS], wl[W][ATT_HEADS];
+    __shared__ const float *wo[W];                   // where warp w left its sums (NULL: it had no tiles)
+    __shared__ uint32_t masks[W][ATT_STAGES];
+    __shared__ long long sums[W];
+    __shared__ Place begin;
+    __shared__ int is_last;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int items = a.kv_heads * a.groups, b = blockIdx.x;
+
+    // This CTA's share: all rows' chunks, in rows' and items' order, are cut
+    // into equal shares. Every CTA adds the chunks up for itself.
+    const int each = (a.n + 32 * W - 1) / (32 * W), r0 = min(a.n, tid * each), r1 = min(a.n, r0 + each);
+    int fault = 0;
+    long long mine = 0;
+    for (int r = r0; r < r1; r++) mine += (long long)chunks_of(row_tokens(a, r, fault), CHUNK) * items;
+    if (fault && b == 0) atomicOr(a.err, fault);
+    long long before = mine;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        qv[j] = lane + 32 * j < a.hs ? q[lane + 32 * j] : 0.0f;
-        o[j] = 0.0f;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xFFFFFFFFu, before, o);
+        if (lane >= o) before += u;
     }
-    for (int t = warp; t <= last; t += ATT_WARPS) {
-        const int blk = div_by(a.c.page, t), p = a.table[(size_t)req * a.c.max_blocks + blk];
-        if (p < 0 || p >= a.c.n_pages) {
-            if (lane == 0) atomicOr(a.err, KV_PAGED_BAD_PAGE);
-            continue;
+    if (lane == 31) sums[warp] = before;
+    __syncthreads();
+    long long all = 0;
+    before -= mine;
+    for (int w = 0; w < W; w++) {
+        if (w == warp) before += all;
+        all += sums[w];
+    }
+    const long long share = (all + gridDim.x - 1) / gridDim.x, first = share * b;
+    if (first >= all) return;
+    if (first >= before && first < before + mine) {
+        long long at = before;
+        for (int r = r0; r < r1; r++) {
+            const int tokens = row_tokens(a, r, fault), ch = chunks_of(tokens, CHUNK);
+            if (first < at + (long long)ch * items) {
+                begin.r = r;
+                begin.tokens = tokens;
+                begin.it = (int)((first - at) / ch);
+                begin.c = (int)((first - at) % ch);
+                begin.left = min(share, all - first);
+                break;
+            }
+            at += (long long)ch * items;
         }
-        const size_t at = p * a.c.page_stride + (t - blk * (int)a.c.page.d) * a.c.token_stride + head;
-        const KV *k = static_cast<const KV *>(a.k_pool) + at, *v = static_cast<const KV *>(a.v_pool) + at;
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (lane + 32 * j < a.hs) s = fmaf(qv[j], kv_get(k + lane + 32 * j), s);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
-        s *= a.scale;
-        const float mn = fmaxf(m, s), f = expf(m - mn), e = expf(s - mn);
-        l = l * f + e;
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = o[j] * f + (lane + 32 * j < a.hs ? e * kv_get(v + lane + 32 * j) : 0.0f);
-        m = mn;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; j++) part[warp][lane + 32 * j] = o[j];
-    if (lane == 0) {
-        part[warp][256] = m;
-        part[warp][257] = l;
     }
     __syncthreads();
-    float mt = -INFINITY, lt = 0.0f;
-    for (int w = 0; w < ATT_WARPS; w++) mt = fmaxf(mt, part[w][256]);
-    for (int w = 0; w < ATT_WARPS; w++)
-        if (part[w][257] > 0.0f) lt += part[w][257] * expf(part[w][256] - mt);
-    for (int d = threadIdx.x; d < a.hs; d += blockDim.x) {
-        float s = 0.0f;
-        for (int w = 0; w < ATT_WARPS; w++)
-            if (part[w][257] > 0.0f) s += part[w][d] * expf(part[w][256] - mt);
-        a.out[((size_t)r * a.heads + h) * a.hs + d] = lt > 0.0f ? s / lt : 0.0f;
+
+    uint8_t *ring = smem + warp * G::RING;
+    const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
+    uint32_t *qf = reinterpret_cast<uint32_t *>(smem + W * G::RING);
+    const int segs = a.hs * (int)sizeof(KV) / 16;
+
+    // ---- loads: tile after tile of this warp, over the items' ends ----
+    Place lp = begin;
+    int lt = warp, l_end = 0, l_tok0 = 0;  // tile of the item in the share, tiles, first token
+    int l_stop = 0;                        // the tokens end here
+    const int *l_table = nullptr;
+    uint64_t l_head = 0;
+    bool l_more = true;
+    auto open_item = [&]() {
+        l_tok0 = lp.c * CHUNK;
+        l_stop = min(lp.tokens, (lp.c + lp.span(CHUNK)) * CHUNK);
+        l_end = l_stop > l_tok0 ? (l_stop - l_tok0 + TILE - 1) / TILE : 0;
+        l_table = a.table + (size_t)a.row_request[lp.r] * a.c.max_blocks;
+        l_head = (uint64_t)(lp.it / a.groups) * a.c.head_stride;
+    };
+    uint64_t nx_at = 0;   // where the next tile's token `lane` lies
+    bool nx_ok = false, nx_any = false;
+    int nx_page = -1, nx_place = 0;
+    // looks up the pages of the next tile: token `lane` of it
+    auto look = [&]() {
+        while (l_more && lt >= l_end) {
+            lp.next(a, CHUNK, items);
+            if (lp.left <= 0) {
+                l_more = false;
+            } else {
+                lt = warp;
+                open_item();
+            }
+        }
+        nx_any = l_more;
+        nx_page = -1;
+        nx_ok = false;
+        if (!l_more) return;
+        const int tok = l_tok0 + lt * TILE + lane;
+        if (lane < TILE && tok < l_stop) {
+            const int blk = div_by(a.c.page, tok);
+            nx_place = tok - blk * (int)a.c.page.d;
+            nx_page = l_table[blk];
+            nx_ok = true;
+        }
+        nx_at = l_head;
+        lt += W;
+    };
+    auto issue = [&](int slot) {
+        if (nx_any) {
+            uint64_t at = nx_at;
+            if (nx_ok && (nx_page < 0 || nx_page >= a.c.n_pages)) {
+                atomicOr(a.err, KV_PAGED_BAD_PAGE);
+                nx_ok = false;
+            }
+            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, nx_ok);
+            if (nx_ok) at += (uint64_t)nx_page * a.c.page_stride + (uint64_t)nx_place * a.c.token_stride;
+            if (lane == 0) masks[warp][slot] = mask;
+            const uint32_t dst0 = ring_s + slot * G::STAGE;
+#pragma unroll
+            for (int i = 0; i < TILE * G::SEGS / 32; i++) {
+                const int idx = lane + 32 * i, key = idx / G::SEGS, seg = idx % G::SEGS;
+                const uint64_t from = __shfl_sync(0xFFFFFFFFu, at, key);
+                const bool ok = ((mask >> key) & 1u) && seg < segs;
+                const int bytes = ok ? 16 : 0;
+                const uint64_t e = ok ? from + seg * (16 / sizeof(KV)) : 0;
+                const uint32_t dst = dst0 + key * G::ROW + seg * 16;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                             "l"(static_cast<const KV *>(a.k_pool) + e), "r"(bytes)
+                             : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE * G::ROW),
+                             "l"(static_cast<const KV *>(a.v_pool) + e), "r"(bytes)
+                             : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (nx_any) look();
+    };
+    open_item();
+    look();
+#pragma unroll
+    for (int s = 0; s < ATT_STAGES; s++) issue(s);
+
+    // ---- items ----
+    Place cp = begin;
+    int slot = 0;
+    while (true) {
+        const int span = cp.span(CHUNK), tok0 = cp.c * CHUNK, stop = min(cp.tokens, (cp.c + span) * CHUNK);
+        const int tiles = stop > tok0 ? (stop - tok0 + TILE - 1) / TILE : 0;
+        const int kvh = cp.it / a.groups, grp = cp.it - kvh * a.groups, group = a.heads / a.kv_heads;
+        const int h0 = kvh * group + grp * a.group_heads;
+        const int H = min(a.group_heads, group - grp * a.group_heads);
+        // q as the products' left operand; head h by warp h mod W
+        for (int h = warp; h < ATT_HEADS; h += W) {
+            const float *q = a.q + (size_t)cp.r * a.q_stride + (size_t)(h0 + h) * a.hs;
+            const float cq = a.scale * 1.44269504088896f;  // scores in base 2
+            float x[HSP / 32];
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < HSP / 64; i++) {
+                const int d = 2 * lane + 64 * i;
+                const float2 v = h < H && d < a.hs ? *reinterpret_cast<const float2 *>(q + d) : make_float2(0.0f, 0.0f);
+                x[2 * i] = v.x * cq;
+                x[2 * i + 1] = v.y * cq;
+                big = fmaxf(big, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
+            }
+            float unit = 1.0f;
+            if (G::HALF) {
+                // the head's largest entry goes to 2^13 .. 2^14, so that the
+                // lower parts of all that matter stay normal halves
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, o));
+                const int ex = (int)((__float_as_uint(big) >> 23) & 255u) - 127;
+                const int up = big > 0.0f && ex < 128 ? min(100, max(-100, 13 - ex)) : 0;
+                unit = __uint_as_float((uint32_t)(127 - up) << 23);
+                const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+#pragma unroll
+                for (int i = 0; i < HSP / 32; i++) x[i] *= f;
+            }
+            if (lane == 0) row_unit[h] = unit;
+#pragma unroll
+            for (int i = 0; i < HSP / 64; i++) {
+                const int d = 2 * lane + 64 * i;
+                if (G::HALF) {
+                    uint32_t hi, lo;
+                    split_f16(x[2 * i], x[2 * i + 1], hi, lo);
+                    const int kk = d & 15;
+                    uint32_t *f = qf + (d >> 4) * 128 + (4 * h + (kk & 7) / 2) * 4 + (kk >> 3) * 2;
+                    *reinterpret_cast<uint2 *>(f) = make_uint2(hi, lo);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        uint32_t hi, lo;
+                        split_tf32(x[2 * i + j], hi, lo);
+                        const int kk = (d + j) & 7;
+                        uint32_t *f = qf + ((d + j) >> 3) * 128 + (4 * h + (kk & 3)) * 4 + (kk >> 2) * 2;
+                        *reinterpret_cast<uint2 *>(f) = make_uint2(hi, lo);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const float unit = row_unit[g];
+        float o[DT][4], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        int hold = -1;  // the slot of this warp's last tile, refilled after the item's end
+        for (int tile = warp; tile < tiles; tile += W) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(ATT_STAGES - 1) : "memory");
+            __syncwarp();
+            const uint32_t mask = masks[warp][slot];
+            const uint32_t ks_s = ring_s + slot * G::STAGE, vs_s = ks_s + TILE * G::ROW;
+            if (mask != 0u) {
+                float s[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+                if (G::HALF) {
+                    const uint32_t at = ks_s + ((lane >> 4) * 8 + (lane & 7)) * G::ROW + ((lane >> 3) & 1) * 16;
+#pragma unroll
+                    for (int ks = 0; ks < HSP / 16; ks++) {
+                        const uint4 qv = *reinterpret_cast<const uint4 *>(qf + ks * 128 + lane * 4);
+                        const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
+#pragma unroll
+                        for (int j = 0; j < NT / 2; j++) {
+                            uint32_t kb[4];
+                            ldmatrix4(kb, at + 16 * j * G::ROW + ks * 32);
+                            mma_f16(s[2 * j], qa, kb[0], kb[1]);
+                            mma_f16(s[2 * j + 1], qa, kb[2], kb[3]);
+                        }
+                    }
+                } else {
+                    float s2[NT][4];  // the lower parts' products, a second chain
+#pragma unroll
+                    for (int j = 0; j < NT; j++) s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.0f;
+                    const uint32_t at = ks_s + (lane & 7) * G::ROW + (lane >> 3) * 16;
+#pragma unroll
+                    for (int ks = 0; ks < HSP / 16; ks++) {
+                        const uint4 q0 = *reinterpret_cast<const uint4 *>(qf + 2 * ks * 128 + lane * 4);
+                        const uint4 q1 = *reinterpret_cast<const uint4 *>(qf + (2 * ks + 1) * 128 + lane * 4);
+                        const uint32_t qa[4] = {q0.x, q0.y, q0.z, q0.w}, qb[4] = {q1.x, q1.y, q1.z, q1.w};
+#pragma unroll
+                        for (int j = 0; j < NT; j++) {
+                            uint32_t kb[4], hi[4], lo[4];
+                            ldmatrix4(kb, at + 8 * j * G::ROW + ks * 64);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(kb[i]), hi[i], lo[i]);
+                            mma_tf32(s[j], qa, hi[0], hi[1]);
+                            mma_tf32(s2[j], qa, lo[0], lo[1]);
+                            mma_tf32(s[j], qb, hi[2], hi[3]);
+                            mma_tf32(s2[j], qb, lo[2], lo[3]);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; j++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) s[j][i] += s2[j][i];
+                }
+                // head g's scores of tokens 8j + 2 t4 and the next one
+                float top = -INFINITY, p[NT][2];
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        p[j][i] = (s[j][i] + s[j][i + 2]) * unit;
+                        if (!((mask >> (8 * j + 2 * t4 + i)) & 1u)) p[j][i] = -INFINITY;
+                        top = fmaxf(top, p[j][i]);
+                    }
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                if (__any_sync(0xFFFFFFFFu, top > m)) {
+                    const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
+                    m = mn;
+                    l *= f;
+#pragma unroll
+                    for (int i = 0; i < DT; i++) {
+                        o[i][0] *= f;
+                        o[i][1] *= f;
+                        o[i][2] *= f;
+                        o[i][3] *= f;
+                    }
+                }
+                // 2^12 p in a half cache's products: its parts' smallest
+                // steps are then 2^-36 of the largest p
+                const float base = (m == -INFINITY ? 0.0f : m) - (G::HALF ? 12.0f : 0.0f);
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        p[j][i] = exp2_fast(p[j][i] - base);
+                        l += p[j][i];
+                    }
+                }
+                if (G::HALF) {
+#pragma unroll
+                    for (int kb = 0; kb < TILE / 16; kb++) {
+                        uint32_t pa[4];
+                        split_f16(p[2 * kb][0], p[2 * kb][1], pa[0], pa[1]);
+                        split_f16(p[2 * kb + 1][0], p[2 * kb + 1][1], pa[2], pa[3]);
+                        const uint32_t at = vs_s + (16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7)) * G::ROW + (lane >> 4) * 16;
+#pragma unroll
+                        for (int i = 0; i < DT / 2; i++) {
+                            uint32_t vb[4];
+                            ldmatrix4_t(vb, at + i * 32);
+                            mma_f16(o[2 * i], pa, vb[0], vb[1]);
+                            mma_f16(o[2 * i + 1], pa, vb[2], vb[3]);
+                        }
+                    }
+                } else {
+                    // inner index t4 stands for token 2 t4, t4 + 4 for 2 t4 + 1;
+                    // column g of o[4c + i] for channel 32c + 4g + i
+#pragma unroll
+                    for (int kb = 0; kb < NT; kb++) {
+                        uint32_t pa[4];
+                        split_tf32(p[kb][0], pa[0], pa[1]);
+                        split_tf32(p[kb][1], pa[2], pa[3]);
+                        const float *v0 = reinterpret_cast<const float *>(
+                            ring + slot * G::STAGE + (TILE + 8 * kb + 2 * t4) * G::ROW + g * 16);
+#pragma unroll
+                        for (int c = 0; c < HSP / 32; c++) {
+                            const float4 x = *reinterpret_cast<const float4 *>(v0 + 32 * c);
+                            const float4 y = *reinterpret_cast<const float4 *>(v0 + G::ROW / 4 + 32 * c);
+                            const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                uint32_t xh, xl, yh, yl;
+                                split_tf32(xs[i], xh, xl);
+                                split_tf32(ys[i], yh, yl);
+                                mma_tf32(o[4 * c + i], pa, xh, yh);
+                                mma_tf32(o[4 * c + i], pa, xl, yl);
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (tile + W < tiles) {
+                issue(slot);
+            } else {
+                hold = slot;
+            }
+            slot = slot + 1 == ATT_STAGES ? 0 : slot + 1;
+        }
+        // the warps' sums, each in the slot of its last tile
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+        if (hold >= 0) {
+            float *dst = reinterpret_cast<float *>(ring + hold * G::STAGE) + g * G::OROW;
+#pragma unroll
+            for (int i = 0; i < DT; i++) {
+                const float x = o[i][0] + o[i][2], y = o[i][1] + o[i][3];
+                if (G::HALF) {
+                    *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t4) = make_float2(x, y);
+                } else {
+                    dst[32 * (i / 4) + 8 * t4 + (i & 3)] = x;
+                    dst[32 * (i / 4) + 8 * t4 + 4 + (i & 3)] = y;
+                }
+            }
+        }
+        if (t4 == 0) {
+            wm[warp][g] = m;
+            wl[warp][g] = hold >= 0 ? l : 0.0f;
+        }
+        if (lane == 0) wo[warp] = hold >= 0 ? reinterpret_cast<const float *>(ring + hold * G::STAGE) : nullptr;
+        __syncthreads();
+        const int ch = chunks_of(cp.tokens, CHUNK);
+        const bool whole = cp.c == 0 && span == ch;
+        const int F4 = a.hs >> 2;
+        float *part = a.part + (size_t)(2 * b + (cp.c == 0 ? 1 : 0)) * ATT_HEADS * (HSP + 2);
+        float *out = a.out + ((size_t)cp.r * a.heads + h0) * a.hs;
+        for (int i = tid; i < H * F4; i += 32 * W) {
+            const int h = i / F4, d = 4 * (i - h * F4);
+            float mt = -INFINITY, lt = 0.0f;
+#pragma unroll
+            for (int w = 0; w < W; w++)
+                if (wl[w][h] != 0.0f) mt = fmaxf(mt, wm[w][h]);
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < W; w++) {
+                if (wl[w][h] != 0.0f) {
+                    const float f = mt == -INFINITY ? 1.0f : exp2_fast(wm[w][h] - mt);
+                    const float4 v = *reinterpret_cast<const float4 *>(wo[w] + h * G::OROW + d);
+                    lt = fmaf(f, wl[w][h], lt);
+                    s.x = fmaf(f, v.x, s.x);
+                    s.y = fmaf(f, v.y, s.y);
+                    s.z = fmaf(f, v.z, s.z);
+                    s.w = fmaf(f, v.w, s.w);
+                }
+            }
+            if (whole) {
+                const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
+                *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+            } else {
+                float *ph = part + (size_t)h * (HSP + 2);
+                *reinterpret_cast<float2 *>(ph + d) = make_float2(s.x, s.y);
+                *reinterpret_cast<float2 *>(ph + d + 2) = make_float2(s.z, s.w);
+                if (d == 0) *reinterpret_cast<float2 *>(ph + HSP) = make_float2(mt, lt);
+            }
+        }
+        if (!whole) {
+            // the item's chunks begin at `item0` of all rows' chunks; the
+            // last of its CTAs to arrive joins the parts in their order
+            const long long item0 = first + (min(share, all - first) - cp.left) - cp.c;
+            const int b0 = (int)(item0 / share), parts = (int)((item0 + ch - 1) / share) - b0 + 1;
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) is_last = atomicInc(a.arrived + b0, (unsigned)parts - 1) == (unsigned)parts - 1;
+            __syncthreads();
+            if (is_last) {
+                __threadfence();
+                for (int i = tid; i < H * F4; i += 32 * W) {
+                    const int h = i / F4, d = 4 * (i - h * F4);
+                    float mt = -INFINITY, lt = 0.0f;
+                    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                    for (int j = 0; j < parts; j++) {
+                        const float *ph = a.part + ((size_t)(2 * (b0 + j) + (j == 0 ? 1 : 0)) * ATT_HEADS + h) * (HSP + 2);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(ph + HSP));
+                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(ph + d));
+                        const float2 y = __ldcg(reinterpret_cast<const float2 *>(ph + d + 2));
+                        if (ml.y != 0.0f) {
+                            const float mn = fmaxf(mt, ml.x);
+                            const float fo = mn == -INFINITY ? 1.0f : exp2_fast(mt - mn);
+                            const float fn = mn == -INFINITY ? 1.0f : exp2_fast(ml.x - mn);
+                            mt = mn;
+                            lt = lt * fo + ml.y * fn;
+                            s.x = s.x * fo + x.x * fn;
+                            s.y = s.y * fo + x.y * fn;
+                            s.z = s.z * fo + y.x * fn;
+                            s.w = s.w * fo + y.y * fn;
+                        }
+                    }
+                    const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
+                    *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+                }
+            }
+        }
+        cp.next(a, CHUNK, items);
+        if (cp.left <= 0) break;
+        __syncthreads();  // the sums are read: their slots may be filled
+        if (hold >= 0) issue(hold);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 }  // namespace kvp
@@ -393,8 +892,13 @@ struct KvPaged {
     KvPagedShape s;
     kvp::Cache c;
     int device, sms;
-    unsigned *arrived;  // device: map's arrivals
-    int *err;           // device: error bits
+    int hsp;            // attend: head size that the kernel is built for, 64, 128 or 256
+    int grid;           // attend: CTAs, as many as are resident at once
+    uint8_t *scratch;   // device: all of the below
+    int *err;           // error bits
+    unsigned *map_arrived;
+    unsigned *arrived;  // attend: [grid]
+    float *part;        // attend: [2 * grid][ATT_HEADS][hsp + 2]
     char msg[256];
 };
 
@@ -470,6 +974,22 @@ static int launched(KvPaged *kv, const char *what)
     return 0;
 }
 
+// The attention kernel of a handle, its dynamic shared memory, and the call of
+// `use` with them.
+template <typename F>
+static auto with_attend(const KvPaged *kv, F use)
+{
+    using namespace kvp;
+    if (kv->s.type == 1) {
+        if (kv->hsp == 64) return use(attend_kernel<__half, 64>, Geo<__half, 64>::SMEM);
+        if (kv->hsp == 128) return use(attend_kernel<__half, 128>, Geo<__half, 128>::SMEM);
+        return use(attend_kernel<__half, 256>, Geo<__half, 256>::SMEM);
+    }
+    if (kv->hsp == 64) return use(attend_kernel<float, 64>, Geo<float, 64>::SMEM);
+    if (kv->hsp == 128) return use(attend_kernel<float, 128>, Geo<float, 128>::SMEM);
+    return use(attend_kernel<float, 256>, Geo<float, 256>::SMEM);
+}
+
 static bool off16(const void *p)
 {
     return ((uintptr_t)p & 15) != 0;
@@ -503,11 +1023,28 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
     if (e == cudaSuccess) {
         OnDevice on(device);
         e = on.ok ? cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device) : cudaErrorInvalidDevice;
-        if (e == cudaSuccess) e = cudaMalloc(&kv->arrived, 256);
-        if (e == cudaSuccess) e = cudaMemset(kv->arrived, 0, 256);
+        kv->hsp = s.head_size <= 64 ? 64 : s.head_size <= 128 ? 128 : 256;
+        if (e == cudaSuccess) {
+            e = with_attend(kv, [&](auto kernel, int smem) {
+                int per_sm = 0;
+                cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                if (x == cudaSuccess)
+                    x = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, 32 * kvp::ATT_WARPS, smem);
+                kv->grid = per_sm * kv->sms;
+                return x == cudaSuccess && per_sm < 1 ? cudaErrorInvalidConfiguration : x;
+            });
+        }
+        const size_t flags = 256 + (((size_t)kv->grid * 4 + 255) & ~(size_t)255);
+        const size_t parts = (size_t)2 * kv->grid * kvp::ATT_HEADS * (kv->hsp + 2) * 4;
+        if (e == cudaSuccess) e = cudaMalloc(&kv->scratch, flags + parts);
+        if (e == cudaSuccess) e = cudaMemset(kv->scratch, 0, flags);
         if (e == cudaSuccess)
             e = cudaFuncSetAttribute(kvp::map_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      3 * (KV_PAGED_MAX_REQUESTS + 1) * 4);
+        kv->err = (int *)kv->scratch;
+        kv->map_arrived = (unsigned *)kv->scratch + 32;
+        kv->arrived = (unsigned *)(kv->scratch + 256);
+        kv->part = (float *)(kv->scratch + flags);
         if (e == cudaSuccess) e = cudaDeviceSynchronize();
     }
     if (e != cudaSuccess) {
@@ -516,16 +1053,15 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
         kv_paged_close(kv);
         return nullptr;
     }
-    kv->err = (int *)(kv->arrived + 32);
     return kv;
 }
 
 extern "C" void kv_paged_close(KvPaged *kv)
 {
     if (kv == nullptr) return;
-    if (kv->arrived) {
+    if (kv->scratch) {
         OnDevice on(kv->device);
-        cudaFree(kv->arrived);
+        cudaFree(kv->scratch);
     }
     delete kv;
 }
@@ -563,7 +1099,7 @@ extern "C" int kv_paged_map(KvPaged *kv, const int *len, const int *start, const
     OnDevice on(kv->device);
     if (!on.ok) return refuse(kv, "CUDA device cannot be used.");
     kvp::MapArgs a = {len, start, end, n, table, free_pages, n_free, n_free_out, max_rows, row_request, row_pos,
-                      row_slot, row0, kv->c, kv->arrived, kv->err};
+                      row_slot, row0, kv->c, kv->map_arrived, kv->err};
     int grid = (max_rows + 4 * kvp::MAP_THREADS - 1) / (4 * kvp::MAP_THREADS);
     if (grid > 2 * kv->sms) grid = 2 * kv->sms;
     if (grid < 1) grid = 1;
@@ -631,14 +1167,32 @@ extern "C" int kv_paged_attend(KvPaged *kv, const float *q, const void *k_pool, 
     if (n == 0) return 1;
     OnDevice on(kv->device);
     if (!on.ok) return refuse(kv, "CUDA device cannot be used.");
-    kvp::AttendArgs a = {q, k_pool, v_pool, table, row_request, row_pos, n, n_requests, s.n_heads, s.n_kv_heads,
-                         s.head_size, scale, out, q_stride, kv->c, kv->err};
+    kvp::AttendArgs a;
+    a.q = q;
+    a.k_pool = k_pool;
+    a.v_pool = v_pool;
+    a.table = table;
+    a.row_request = row_request;
+    a.row_pos = row_pos;
+    a.n = n;
+    a.n_requests = n_requests;
+    a.heads = s.n_heads;
+    a.kv_heads = s.n_kv_heads;
+    a.hs = s.head_size;
+    const int group = s.n_heads / s.n_kv_heads;
+    a.groups = (group + kvp::ATT_HEADS - 1) / kvp::ATT_HEADS;
+    a.group_heads = (group + a.groups - 1) / a.groups;
+    a.scale = scale;
+    a.out = out;
+    a.q_stride = q_stride;
+    a.c = kv->c;
+    a.part = kv->part;
+    a.arrived = kv->arrived;
+    a.err = kv->err;
     cudaGetLastError();
-    const dim3 grid(s.n_heads, n);
-    if (s.type == 1) {
-        kvp::attend_kernel<__half><<<grid, 32 * kvp::ATT_WARPS, 0, (cudaStream_t)stream>>>(a);
-    } else {
-        kvp::attend_kernel<float><<<grid, 32 * kvp::ATT_WARPS, 0, (cudaStream_t)stream>>>(a);
-    }
+    with_attend(kv, [&](auto kernel, int smem) {
+        kernel<<<kv->grid, 32 * kvp::ATT_WARPS, smem, (cudaStream_t)stream>>>(a);
+        return 0;
+    });
     return launched(kv, "attend");
 }
