@@ -392,6 +392,16 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
 
+// o = o f + the sum of both halves of a tile's product. The running sums are
+// kept outside the tensor cores, whose accumulators cut bits off instead of
+// rounding: over a thousand tokens that adds up to 2e-6 of the result, always
+// towards zero.
+__device__ __forceinline__ void add_tile(float (&o)[2], const float (&x)[4], float f)
+{
+    o[0] = fmaf(o[0], f, x[0] + x[2]);
+    o[1] = fmaf(o[1], f, x[1] + x[3]);
+}
+
 // Row r's visible tokens, -1 for a row that is passed over.
 __device__ __forceinline__ int row_tokens(const AttendArgs &a, int r, int &fault)
 {
@@ -641,9 +651,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
         }
         __syncthreads();
         const float unit = row_unit[g];
-        float o[DT][4], m = -INFINITY, l = 0.0f;
+        float o[DT][2], m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
         int hold = -1;  // the slot of this warp's last tile, refilled after the item's end
         for (int tile = warp; tile < tiles; tile += W) {
             asm volatile("cp.async.wait_group %0;" ::"n"(ATT_STAGES - 1) : "memory");
@@ -708,18 +718,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                if (__any_sync(0xFFFFFFFFu, top > m)) {
-                    const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
-                    m = mn;
-                    l *= f;
-#pragma unroll
-                    for (int i = 0; i < DT; i++) {
-                        o[i][0] *= f;
-                        o[i][1] *= f;
-                        o[i][2] *= f;
-                        o[i][3] *= f;
-                    }
-                }
+                const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
+                m = mn;
+                l *= f;
                 // 2^12 p in a half cache's products: its parts' smallest
                 // steps are then 2^-36 of the largest p
                 const float base = (m == -INFINITY ? 0.0f : m) - (G::HALF ? 12.0f : 0.0f);
@@ -742,8 +743,11 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
                         for (int i = 0; i < DT / 2; i++) {
                             uint32_t vb[4];
                             ldmatrix4_t(vb, at + i * 32);
-                            mma_f16(o[2 * i], pa, vb[0], vb[1]);
-                            mma_f16(o[2 * i + 1], pa, vb[2], vb[3]);
+                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_f16(x, pa, vb[0], vb[1]);
+                            mma_f16(y, pa, vb[2], vb[3]);
+                            add_tile(o[2 * i], x, kb == 0 ? f : 1.0f);
+                            add_tile(o[2 * i + 1], y, kb == 0 ? f : 1.0f);
                         }
                     }
                 } else {
@@ -766,8 +770,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
                                 uint32_t xh, xl, yh, yl;
                                 split_tf32(xs[i], xh, xl);
                                 split_tf32(ys[i], yh, yl);
-                                mma_tf32(o[4 * c + i], pa, xh, yh);
-                                mma_tf32(o[4 * c + i], pa, xl, yl);
+                                float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma_tf32(s4, pa, xl, yl);
+                                mma_tf32(s4, pa, xh, yh);
+                                add_tile(o[4 * c + i], s4, kb == 0 ? f : 1.0f);
                             }
                         }
                     }
@@ -788,7 +794,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
             float *dst = reinterpret_cast<float *>(ring + hold * G::STAGE) + g * G::OROW;
 #pragma unroll
             for (int i = 0; i < DT; i++) {
-                const float x = o[i][0] + o[i][2], y = o[i][1] + o[i][3];
+                const float x = o[i][0], y = o[i][1];
                 if (G::HALF) {
                     *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t4) = make_float2(x, y);
                 } else {
