@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
 // (keys and values, about 9 KB) are in flight by 16-byte async copies, with
 // the page numbers of the tile after them; a warp waits for no other before
 // an item's end. Tokens that a row may not see are zero-filled, never read.
-constexpr int ATT_WARPS = 4, ATT_STAGES = 3, ATT_HEADS = 8;
+constexpr int ATT_WARPS = 4, ATT_HEADS = 8;
 
 template <typename KV, int HSP>
 struct Geo {
@@ -318,7 +318,9 @@ struct Geo {
     static constexpr int CHUNK = ATT_WARPS * TILE;   // tokens: the unit in which work is shared out
     static constexpr int ROW = HSP * (int)sizeof(KV) + 16;  // bytes; 16 past a multiple of 128: no bank conflicts
     static constexpr int STAGE = 2 * TILE * ROW;
-    static constexpr int RING = ATT_STAGES * STAGE;
+    static constexpr int STAGES = HSP == 256 ? 3 : 2;
+    static constexpr int CTAS = HSP == 256 ? 1 : 3;  // per SM, as shared memory allows
+    static constexpr int RING = STAGES * STAGE;
     static constexpr int SEGS = HSP * (int)sizeof(KV) / 16;  // 16-byte pieces of a token's head
     static constexpr int QFRAG = (HALF ? HSP / 16 : HSP / 8) * 512;
     static constexpr int SMEM = ATT_WARPS * RING + QFRAG;
@@ -336,7 +338,7 @@ struct AttendArgs {
     float *out;
     uint64_t q_stride;
     Cache c;
-    float *part;        // [2 * grid][ATT_HEADS][HSP + 2]: sums, then maximum and weight
+    float *part;        // [2 * grid][ATT_HEADS][HSP + 4]: sums, then maximum and weight
     unsigned *arrived;  // [grid]: parts of the item that begins in CTA b and ends in another; wraps to 0 by itself
     int *err;
 };
@@ -402,10 +404,10 @@ __device__ __forceinline__ void add_tile(float (&o)[2], const float (&x)[4], flo
     o[1] = fmaf(o[1], f, x[1] + x[3]);
 }
 
-// Row r's visible tokens, -1 for a row that is passed over.
-__device__ __forceinline__ int row_tokens(const AttendArgs &a, int r, int &fault)
+// The visible tokens of a row of request `req` at position `last`, -1 for a
+// row that is passed over.
+__device__ __forceinline__ int row_tokens(const AttendArgs &a, int req, int last, int &fault)
 {
-    const int req = a.row_request[r], last = a.row_pos[r];
     if (req < 0) return -1;
     if (req >= a.n_requests) {
         fault = KV_PAGED_BAD_ROW;
@@ -424,11 +426,20 @@ __host__ __device__ __forceinline__ int chunks_of(int tokens, int chunk)
     return tokens < 0 ? 0 : tokens == 0 ? 1 : (tokens - 1) / chunk + 1;
 }
 
-// A place in a CTA's share of the work: chunk `c` of item `it` of row r.
+// A place in a CTA's share of the work: chunk `c` of item `it` of row r. The
+// next row's numbers are loaded a row ahead.
 struct Place {
-    int r, it, tokens, c;
+    int r, it, tokens, req, c;
+    int next_req, next_pos;
     long long left;  // chunks of the CTA's share from here on
 
+    __device__ __forceinline__ void ahead(const AttendArgs &a)
+    {
+        if (r + 1 < a.n) {
+            next_req = a.row_request[r + 1];
+            next_pos = a.row_pos[r + 1];
+        }
+    }
     // chunks of this item in the share
     __device__ __forceinline__ int span(int chunk) const
     {
@@ -442,19 +453,26 @@ struct Place {
         c = 0;
         if (++it < items || left <= 0) return;
         it = 0;
-        int unused;
+        int unused = 0;
         do {
             if (++r >= a.n) {  // not while the rows stay as they were counted
                 left = 0;
                 return;
             }
-            tokens = row_tokens(a, r, unused);
+            req = next_req;
+            tokens = row_tokens(a, next_req, next_pos, unused);
+            ahead(a);
         } while (tokens < 0);
     }
 };
 
+// A part of an item that other CTAs hold the rest of.
+struct Part {
+    int r, h0, heads, b0, parts;  // the item's first CTA, and how many hold it (0: no such part)
+};
+
 template <typename KV, int HSP>
-__global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs a)
+__global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_kernel(const AttendArgs a)
 {
     using G = Geo<KV, HSP>;
     constexpr int TILE = G::TILE, CHUNK = G::CHUNK, W = ATT_WARPS, NT = TILE / 8, DT = HSP / 8;
@@ -462,10 +480,11 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
     __shared__ float row_unit[ATT_HEADS];            // score = product * row_unit
     __shared__ float wm[W][ATT_HEADS], wl[W][ATT_HEADS];
     __shared__ const float *wo[W];                   // where warp w left its sums (NULL: it had no tiles)
-    __shared__ uint32_t masks[W][ATT_STAGES];
+    __shared__ uint32_t masks[W][G::STAGES];
     __shared__ long long sums[W];
     __shared__ Place begin;
-    __shared__ int is_last;
+    __shared__ Part pend[2];  // the share's first item, begun by another CTA, and its last, ended by another
+    __shared__ int is_last[2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int items = a.kv_heads * a.groups, b = blockIdx.x;
 
@@ -474,7 +493,8 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
     const int each = (a.n + 32 * W - 1) / (32 * W), r0 = min(a.n, tid * each), r1 = min(a.n, r0 + each);
     int fault = 0;
     long long mine = 0;
-    for (int r = r0; r < r1; r++) mine += (long long)chunks_of(row_tokens(a, r, fault), CHUNK) * items;
+    for (int r = r0; r < r1; r++)
+        mine += (long long)chunks_of(row_tokens(a, a.row_request[r], a.row_pos[r], fault), CHUNK) * items;
     if (fault && b == 0) atomicOr(a.err, fault);
     long long before = mine;
 #pragma unroll
@@ -495,13 +515,15 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
     if (first >= before && first < before + mine) {
         long long at = before;
         for (int r = r0; r < r1; r++) {
-            const int tokens = row_tokens(a, r, fault), ch = chunks_of(tokens, CHUNK);
+            const int tokens = row_tokens(a, a.row_request[r], a.row_pos[r], fault), ch = chunks_of(tokens, CHUNK);
             if (first < at + (long long)ch * items) {
                 begin.r = r;
+                begin.req = a.row_request[r];
                 begin.tokens = tokens;
                 begin.it = (int)((first - at) / ch);
                 begin.c = (int)((first - at) % ch);
                 begin.left = min(share, all - first);
+                begin.ahead(a);
                 break;
             }
             at += (long long)ch * items;
@@ -525,7 +547,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
         l_tok0 = lp.c * CHUNK;
         l_stop = min(lp.tokens, (lp.c + lp.span(CHUNK)) * CHUNK);
         l_end = l_stop > l_tok0 ? (l_stop - l_tok0 + TILE - 1) / TILE : 0;
-        l_table = a.table + (size_t)a.row_request[lp.r] * a.c.max_blocks;
+        l_table = a.table + (size_t)lp.req * a.c.max_blocks;
         l_head = (uint64_t)(lp.it / a.groups) * a.c.head_stride;
     };
     uint64_t nx_at = 0;   // where the next tile's token `lane` lies
@@ -589,29 +611,41 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
     open_item();
     look();
 #pragma unroll
-    for (int s = 0; s < ATT_STAGES; s++) issue(s);
+    for (int s = 0; s < G::STAGES; s++) issue(s);
 
-    // ---- items ----
-    Place cp = begin;
-    int slot = 0;
-    while (true) {
-        const int span = cp.span(CHUNK), tok0 = cp.c * CHUNK, stop = min(cp.tokens, (cp.c + span) * CHUNK);
-        const int tiles = stop > tok0 ? (stop - tok0 + TILE - 1) / TILE : 0;
-        const int kvh = cp.it / a.groups, grp = cp.it - kvh * a.groups, group = a.heads / a.kv_heads;
-        const int h0 = kvh * group + grp * a.group_heads;
-        const int H = min(a.group_heads, group - grp * a.group_heads);
-        // q as the products' left operand; head h by warp h mod W
-        for (int h = warp; h < ATT_HEADS; h += W) {
-            const float *q = a.q + (size_t)cp.r * a.q_stride + (size_t)(h0 + h) * a.hs;
-            const float cq = a.scale * 1.44269504088896f;  // scores in base 2
+    // ---- q: head h of an item by warp h mod W; loaded an item ahead ----
+    float2 qn[ATT_HEADS / W][HSP / 64];
+    const int group = a.heads / a.kv_heads;
+    auto heads_of = [&](const Place &p, int &h0, int &H) {
+        const int kvh = p.it / a.groups, grp = p.it - kvh * a.groups;
+        h0 = kvh * group + grp * a.group_heads;
+        H = min(a.group_heads, group - grp * a.group_heads);
+    };
+    auto load_q = [&](const Place &p) {
+        int h0, H;
+        heads_of(p, h0, H);
+#pragma unroll
+        for (int k = 0; k < ATT_HEADS / W; k++) {
+            const int h = warp + k * W;
+            const float *q = a.q + (size_t)p.r * a.q_stride + (size_t)(h0 + h) * a.hs;
+#pragma unroll
+            for (int i = 0; i < HSP / 64; i++) {
+                const int d = 2 * lane + 64 * i;
+                qn[k][i] = h < H && d < a.hs ? __ldg(reinterpret_cast<const float2 *>(q + d)) : make_float2(0.0f, 0.0f);
+            }
+        }
+    };
+    auto store_q = [&]() {
+        const float cq = a.scale * 1.44269504088896f;  // scores in base 2
+#pragma unroll
+        for (int k = 0; k < ATT_HEADS / W; k++) {
+            const int h = warp + k * W;
             float x[HSP / 32];
             float big = 0.0f;
 #pragma unroll
             for (int i = 0; i < HSP / 64; i++) {
-                const int d = 2 * lane + 64 * i;
-                const float2 v = h < H && d < a.hs ? *reinterpret_cast<const float2 *>(q + d) : make_float2(0.0f, 0.0f);
-                x[2 * i] = v.x * cq;
-                x[2 * i + 1] = v.y * cq;
+                x[2 * i] = qn[k][i].x * cq;
+                x[2 * i + 1] = qn[k][i].y * cq;
                 big = fmaxf(big, fmaxf(fabsf(x[2 * i]), fabsf(x[2 * i + 1])));
             }
             float unit = 1.0f;
@@ -649,14 +683,30 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
                 }
             }
         }
-        __syncthreads();
+    };
+
+    // ---- items ----
+    Place cp = begin;
+    int slot = 0;
+    if (tid < 2) pend[tid].parts = 0;
+    load_q(cp);
+    store_q();
+    __syncthreads();
+    while (true) {
+        const int span = cp.span(CHUNK), tok0 = cp.c * CHUNK, stop = min(cp.tokens, (cp.c + span) * CHUNK);
+        const int tiles = stop > tok0 ? (stop - tok0 + TILE - 1) / TILE : 0;
+        int h0, H;
+        heads_of(cp, h0, H);
+        Place np = cp;
+        np.next(a, CHUNK, items);
+        if (np.left > 0) load_q(np);
         const float unit = row_unit[g];
         float o[DT][2], m = -INFINITY, l = 0.0f;
 #pragma unroll
         for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
         int hold = -1;  // the slot of this warp's last tile, refilled after the item's end
         for (int tile = warp; tile < tiles; tile += W) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(ATT_STAGES - 1) : "memory");
+            asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 1) : "memory");
             __syncwarp();
             const uint32_t mask = masks[warp][slot];
             const uint32_t ks_s = ring_s + slot * G::STAGE, vs_s = ks_s + TILE * G::ROW;
@@ -785,7 +835,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
             } else {
                 hold = slot;
             }
-            slot = slot + 1 == ATT_STAGES ? 0 : slot + 1;
+            slot = slot + 1 == G::STAGES ? 0 : slot + 1;
         }
         // the warps' sums, each in the slot of its last tile
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
@@ -809,10 +859,12 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
         }
         if (lane == 0) wo[warp] = hold >= 0 ? reinterpret_cast<const float *>(ring + hold * G::STAGE) : nullptr;
         __syncthreads();
+        if (np.left > 0) store_q();  // every warp is done with this item's
         const int ch = chunks_of(cp.tokens, CHUNK);
         const bool whole = cp.c == 0 && span == ch;
         const int F4 = a.hs >> 2;
-        float *part = a.part + (size_t)(2 * b + (cp.c == 0 ? 1 : 0)) * ATT_HEADS * (HSP + 2);
+        const int side = cp.c == 0 ? 1 : 0;
+        float *part = a.part + (size_t)(2 * b + side) * ATT_HEADS * (HSP + 4);
         float *out = a.out + ((size_t)cp.r * a.heads + h0) * a.hs;
         for (int i = tid; i < H * F4; i += 32 * W) {
             const int h = i / F4, d = 4 * (i - h * F4);
@@ -837,58 +889,87 @@ __global__ void __launch_bounds__(32 * ATT_WARPS) attend_kernel(const AttendArgs
                 const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
                 *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
             } else {
-                float *ph = part + (size_t)h * (HSP + 2);
-                *reinterpret_cast<float2 *>(ph + d) = make_float2(s.x, s.y);
-                *reinterpret_cast<float2 *>(ph + d + 2) = make_float2(s.z, s.w);
+                float *ph = part + (size_t)h * (HSP + 4);
+                *reinterpret_cast<float4 *>(ph + d) = s;
                 if (d == 0) *reinterpret_cast<float2 *>(ph + HSP) = make_float2(mt, lt);
             }
         }
-        if (!whole) {
-            // the item's chunks begin at `item0` of all rows' chunks; the
-            // last of its CTAs to arrive joins the parts in their order
+        if (!whole && tid == 0) {
+            // the item's chunks begin at `item0` of all rows' chunks
             const long long item0 = first + (min(share, all - first) - cp.left) - cp.c;
-            const int b0 = (int)(item0 / share), parts = (int)((item0 + ch - 1) / share) - b0 + 1;
-            __threadfence();
-            __syncthreads();
-            if (tid == 0) is_last = atomicInc(a.arrived + b0, (unsigned)parts - 1) == (unsigned)parts - 1;
-            __syncthreads();
-            if (is_last) {
-                __threadfence();
-                for (int i = tid; i < H * F4; i += 32 * W) {
-                    const int h = i / F4, d = 4 * (i - h * F4);
-                    float mt = -INFINITY, lt = 0.0f;
-                    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (int j = 0; j < parts; j++) {
-                        const float *ph = a.part + ((size_t)(2 * (b0 + j) + (j == 0 ? 1 : 0)) * ATT_HEADS + h) * (HSP + 2);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(ph + HSP));
-                        const float2 x = __ldcg(reinterpret_cast<const float2 *>(ph + d));
-                        const float2 y = __ldcg(reinterpret_cast<const float2 *>(ph + d + 2));
-                        if (ml.y != 0.0f) {
-                            const float mn = fmaxf(mt, ml.x);
-                            const float fo = mn == -INFINITY ? 1.0f : exp2_fast(mt - mn);
-                            const float fn = mn == -INFINITY ? 1.0f : exp2_fast(ml.x - mn);
-                            mt = mn;
-                            lt = lt * fo + ml.y * fn;
-                            s.x = s.x * fo + x.x * fn;
-                            s.y = s.y * fo + x.y * fn;
-                            s.z = s.z * fo + y.x * fn;
-                            s.w = s.w * fo + y.y * fn;
-                        }
-                    }
-                    const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
-                    *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
-                }
-            }
+            const int b0 = (int)(item0 / share);
+            Part &p = pend[side];
+            p.r = cp.r;
+            p.h0 = h0;
+            p.heads = H;
+            p.b0 = b0;
+            p.parts = (int)((item0 + ch - 1) / share) - b0 + 1;
         }
-        cp.next(a, CHUNK, items);
-        if (cp.left <= 0) break;
-        __syncthreads();  // the sums are read: their slots may be filled
+        if (np.left <= 0) break;
+        cp = np;
+        __syncthreads();  // the sums are read: their slots may be filled; q is there
         if (hold >= 0) issue(hold);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-}
 
+    // ---- parts: the last of an item's CTAs to arrive joins them in their order ----
+    __threadfence();
+    __syncthreads();
+    if (tid < 2) {
+        const Part p = pend[tid];
+        is_last[tid] = p.parts > 0 && atomicInc(a.arrived + p.b0, (unsigned)p.parts - 1) == (unsigned)p.parts - 1;
+    }
+    __syncthreads();
+    for (int k = 0; k < 2; k++) {
+        if (!is_last[k]) continue;
+        __threadfence();
+        const Part p = pend[k];
+        const int F4 = a.hs >> 2;
+        float *out = a.out + ((size_t)p.r * a.heads + p.h0) * a.hs;
+        for (int i = tid; i < p.heads * F4; i += 32 * W) {
+            const int h = i / F4, d = 4 * (i - h * F4);
+            float mt = -INFINITY, lt = 0.0f;
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int j0 = 0; j0 < p.parts; j0 += 8) {
+                float2 ml[8];  // eight parts' loads in flight
+                float4 v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int pj = min(j0 + j, p.parts - 1);
+                    const float *ph = a.part + ((size_t)(2 * (p.b0 + pj) + (pj == 0 ? 1 : 0)) * ATT_HEADS + h) * (HSP + 4);
+                    ml[j] = __ldcg(reinterpret_cast<const float2 *>(ph + HSP));
+                    v[j] = __ldcg(reinterpret_cast<const float4 *>(ph + d));
+                }
+                float mn = mt;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (j0 + j >= p.parts) ml[j].y = 0.0f;
+                    if (ml[j].y != 0.0f) mn = fmaxf(mn, ml[j].x);
+                }
+                const float fo = mn == -INFINITY ? 1.0f : exp2_fast(mt - mn);
+                mt = mn;
+                lt *= fo;
+                s.x *= fo;
+                s.y *= fo;
+                s.z *= fo;
+                s.w *= fo;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (ml[j].y != 0.0f) {
+                        const float f = mn == -INFINITY ? 1.0f : exp2_fast(ml[j].x - mn);
+                        lt = fmaf(f, ml[j].y, lt);
+                        s.x = fmaf(f, v[j].x, s.x);
+                        s.y = fmaf(f, v[j].y, s.y);
+                        s.z = fmaf(f, v[j].z, s.z);
+                        s.w = fmaf(f, v[j].w, s.w);
+                    }
+                }
+            }
+            const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
+            *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+        }
+    }
+}
 }  // namespace kvp
 }  // namespace pk
 
@@ -904,7 +985,7 @@ struct KvPaged {
     int *err;           // error bits
     unsigned *map_arrived;
     unsigned *arrived;  // attend: [grid]
-    float *part;        // attend: [2 * grid][ATT_HEADS][hsp + 2]
+    float *part;        // attend: [2 * grid][ATT_HEADS][hsp + 4]
     char msg[256];
 };
 
@@ -1041,7 +1122,7 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
             });
         }
         const size_t flags = 256 + (((size_t)kv->grid * 4 + 255) & ~(size_t)255);
-        const size_t parts = (size_t)2 * kv->grid * kvp::ATT_HEADS * (kv->hsp + 2) * 4;
+        const size_t parts = (size_t)2 * kv->grid * kvp::ATT_HEADS * (kv->hsp + 4) * 4;
         if (e == cudaSuccess) e = cudaMalloc(&kv->scratch, flags + parts);
         if (e == cudaSuccess) e = cudaMemset(kv->scratch, 0, flags);
         if (e == cudaSuccess)
