@@ -42,7 +42,8 @@ __host__ __device__ __forceinline__ int div_by(const Div &v, int x)
 struct Cache {
     Div page;  // page_tokens
     int n_pages, max_blocks;
-    uint64_t page_stride, token_stride, head_stride;
+    uint64_t page_stride, token_stride, head_stride;  // entries
+    uint32_t page_units, token_units, head_units;     // the same in 16 bytes; a pool has less than 2^32 of them
 };
 
 // ------------------------------------------------------------------ //
@@ -476,12 +477,14 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
 {
     using G = Geo<KV, HSP>;
     constexpr int TILE = G::TILE, CHUNK = G::CHUNK, W = ATT_WARPS, NT = TILE / 8, DT = HSP / 8;
+    constexpr int JT = ATT_HEADS * HSP / 4 / (32 * W);  // pieces of 4 channels of all heads, per thread
     extern __shared__ __align__(16) uint8_t smem[];  // rings, then q
     __shared__ float row_unit[ATT_HEADS];            // score = product * row_unit
     __shared__ float wm[W][ATT_HEADS], wl[W][ATT_HEADS];
     __shared__ const float *wo[W];                   // where warp w left its sums (NULL: it had no tiles)
     __shared__ uint32_t masks[W][G::STAGES];
     __shared__ long long sums[W];
+    __shared__ int tops[W];
     __shared__ Place begin;
     __shared__ Part pend[2];  // the share's first item, begun by another CTA, and its last, ended by another
     __shared__ int is_last[2];
@@ -493,8 +496,17 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
     const int each = (a.n + 32 * W - 1) / (32 * W), r0 = min(a.n, tid * each), r1 = min(a.n, r0 + each);
     int fault = 0;
     long long mine = 0;
-    for (int r = r0; r < r1; r++)
-        mine += (long long)chunks_of(row_tokens(a, a.row_request[r], a.row_pos[r], fault), CHUNK) * items;
+    int req0 = -1, tokens0 = -1;  // this thread's first row
+    int longest = 0;
+    for (int r = r0; r < r1; r++) {
+        const int req = a.row_request[r], tokens = row_tokens(a, req, a.row_pos[r], fault);
+        mine += (long long)chunks_of(tokens, CHUNK) * items;
+        longest = max(longest, chunks_of(tokens, CHUNK));
+        if (r == r0) {
+            req0 = req;
+            tokens0 = tokens;
+        }
+    }
     if (fault && b == 0) atomicOr(a.err, fault);
     long long before = mine;
 #pragma unroll
@@ -502,28 +514,37 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
         const long long u = __shfl_up_sync(0xFFFFFFFFu, before, o);
         if (lane >= o) before += u;
     }
-    if (lane == 31) sums[warp] = before;
+    longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+    if (lane == 31) {
+        sums[warp] = before;
+        tops[warp] = longest;
+    }
     __syncthreads();
     long long all = 0;
     before -= mine;
     for (int w = 0; w < W; w++) {
         if (w == warp) before += all;
         all += sums[w];
+        longest = max(longest, tops[w]);
     }
-    const long long share = (all + gridDim.x - 1) / gridDim.x, first = share * b;
+    // A part costs the CTA that joins it about 0.25 us, a chunk in a GPU that
+    // is not full about 0.6 us, so where all CTAs together would have less,
+    // shares are not smaller than makes both sides equal for the longest item:
+    // c parts of longest / c chunks.
+    const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)__fsqrt_rn(0.4f * longest)), first = share * b;
     if (first >= all) return;
     if (first >= before && first < before + mine) {
         long long at = before;
         for (int r = r0; r < r1; r++) {
-            const int tokens = row_tokens(a, a.row_request[r], a.row_pos[r], fault), ch = chunks_of(tokens, CHUNK);
+            const int req = r == r0 ? req0 : a.row_request[r];
+            const int tokens = r == r0 ? tokens0 : row_tokens(a, req, a.row_pos[r], fault), ch = chunks_of(tokens, CHUNK);
             if (first < at + (long long)ch * items) {
                 begin.r = r;
-                begin.req = a.row_request[r];
+                begin.req = req;
                 begin.tokens = tokens;
                 begin.it = (int)((first - at) / ch);
                 begin.c = (int)((first - at) % ch);
                 begin.left = min(share, all - first);
-                begin.ahead(a);
                 break;
             }
             at += (long long)ch * items;
@@ -538,19 +559,20 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
 
     // ---- loads: tile after tile of this warp, over the items' ends ----
     Place lp = begin;
+    lp.ahead(a);
     int lt = warp, l_end = 0, l_tok0 = 0;  // tile of the item in the share, tiles, first token
     int l_stop = 0;                        // the tokens end here
     const int *l_table = nullptr;
-    uint64_t l_head = 0;
+    uint32_t l_head = 0;
     bool l_more = true;
     auto open_item = [&]() {
         l_tok0 = lp.c * CHUNK;
         l_stop = min(lp.tokens, (lp.c + lp.span(CHUNK)) * CHUNK);
         l_end = l_stop > l_tok0 ? (l_stop - l_tok0 + TILE - 1) / TILE : 0;
         l_table = a.table + (size_t)lp.req * a.c.max_blocks;
-        l_head = (uint64_t)(lp.it / a.groups) * a.c.head_stride;
+        l_head = (uint32_t)(lp.it / a.groups) * a.c.head_units;
     };
-    uint64_t nx_at = 0;   // where the next tile's token `lane` lies
+    uint32_t nx_at = 0;  // where the next tile's token `lane` lies, in 16 bytes
     bool nx_ok = false, nx_any = false;
     int nx_page = -1, nx_place = 0;
     // looks up the pages of the next tile: token `lane` of it
@@ -580,39 +602,34 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
     };
     auto issue = [&](int slot) {
         if (nx_any) {
-            uint64_t at = nx_at;
+            uint32_t at = nx_at;
             if (nx_ok && (nx_page < 0 || nx_page >= a.c.n_pages)) {
                 atomicOr(a.err, KV_PAGED_BAD_PAGE);
                 nx_ok = false;
             }
             const uint32_t mask = __ballot_sync(0xFFFFFFFFu, nx_ok);
-            if (nx_ok) at += (uint64_t)nx_page * a.c.page_stride + (uint64_t)nx_place * a.c.token_stride;
+            if (nx_ok) at += (uint32_t)nx_page * a.c.page_units + (uint32_t)nx_place * a.c.token_units;
             if (lane == 0) masks[warp][slot] = mask;
             const uint32_t dst0 = ring_s + slot * G::STAGE;
 #pragma unroll
             for (int i = 0; i < TILE * G::SEGS / 32; i++) {
                 const int idx = lane + 32 * i, key = idx / G::SEGS, seg = idx % G::SEGS;
-                const uint64_t from = __shfl_sync(0xFFFFFFFFu, at, key);
+                const uint32_t from = __shfl_sync(0xFFFFFFFFu, at, key);
                 const bool ok = ((mask >> key) & 1u) && seg < segs;
                 const int bytes = ok ? 16 : 0;
-                const uint64_t e = ok ? from + seg * (16 / sizeof(KV)) : 0;
+                const uint64_t e = ok ? (uint64_t)(from + seg) * 16 : 0;
                 const uint32_t dst = dst0 + key * G::ROW + seg * 16;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-                             "l"(static_cast<const KV *>(a.k_pool) + e), "r"(bytes)
+                             "l"(static_cast<const uint8_t *>(a.k_pool) + e), "r"(bytes)
                              : "memory");
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE * G::ROW),
-                             "l"(static_cast<const KV *>(a.v_pool) + e), "r"(bytes)
+                             "l"(static_cast<const uint8_t *>(a.v_pool) + e), "r"(bytes)
                              : "memory");
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (nx_any) look();
     };
-    open_item();
-    look();
-#pragma unroll
-    for (int s = 0; s < G::STAGES; s++) issue(s);
-
     // ---- q: head h of an item by warp h mod W; loaded an item ahead ----
     float2 qn[ATT_HEADS / W][HSP / 64];
     const int group = a.heads / a.kv_heads;
@@ -686,10 +703,14 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
     };
 
     // ---- items ----
-    Place cp = begin;
+    Place cp = lp;
     int slot = 0;
     if (tid < 2) pend[tid].parts = 0;
-    load_q(cp);
+    load_q(cp);  // ahead of the tiles: behind them it would wait for all that all CTAs ask for
+    open_item();
+    look();
+#pragma unroll
+    for (int s = 0; s < G::STAGES; s++) issue(s);
     store_q();
     __syncthreads();
     while (true) {
@@ -913,6 +934,8 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
     asm volatile("cp.async.wait_all;" ::: "memory");
 
     // ---- parts: the last of an item's CTAs to arrive joins them in their order ----
+    __syncthreads();
+    if (pend[0].parts == 0 && pend[1].parts == 0) return;
     __threadfence();
     __syncthreads();
     if (tid < 2) {
@@ -924,52 +947,99 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
         if (!is_last[k]) continue;
         __threadfence();
         const Part p = pend[k];
-        const int F4 = a.hs >> 2;
+        const int F4 = a.hs >> 2, bytes = p.heads * (HSP + 4) * 4, fit = W * G::RING / bytes;
         float *out = a.out + ((size_t)p.r * a.heads + p.h0) * a.hs;
-        for (int i = tid; i < p.heads * F4; i += 32 * W) {
-            const int h = i / F4, d = 4 * (i - h * F4);
-            float mt = -INFINITY, lt = 0.0f;
-            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            for (int j0 = 0; j0 < p.parts; j0 += 8) {
-                float2 ml[8];  // eight parts' loads in flight
-                float4 v[8];
+        const float *src0 = a.part + (size_t)2 * p.b0 * ATT_HEADS * (HSP + 4);
+        // part j of the item: the first CTA's is its last item, the others' their first
+        auto part_of = [&](int j) { return src0 + (size_t)(2 * j + (j == 0 ? 1 : 0)) * ATT_HEADS * (HSP + 4); };
+        float4 s[JT];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int pj = min(j0 + j, p.parts - 1);
-                    const float *ph = a.part + ((size_t)(2 * (p.b0 + pj) + (pj == 0 ? 1 : 0)) * ATT_HEADS + h) * (HSP + 4);
-                    ml[j] = __ldcg(reinterpret_cast<const float2 *>(ph + HSP));
-                    v[j] = __ldcg(reinterpret_cast<const float4 *>(ph + d));
-                }
-                float mn = mt;
+        for (int c = 0; c < JT; c++) s[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j0 = 0; j0 < p.parts; j0 += fit) {
+            // as many parts as fit, all their loads in flight at once; a warp takes every W-th part
+            const int nj = min(fit, p.parts - j0);
+            __syncthreads();
+            float2 ml[ATT_HEADS / W][2];  // heads warp, warp + W: the first 64 parts' maxima and weights
+            if (j0 == 0) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (j0 + j >= p.parts) ml[j].y = 0.0f;
-                    if (ml[j].y != 0.0f) mn = fmaxf(mn, ml[j].x);
-                }
-                const float fo = mn == -INFINITY ? 1.0f : exp2_fast(mt - mn);
-                mt = mn;
-                lt *= fo;
-                s.x *= fo;
-                s.y *= fo;
-                s.z *= fo;
-                s.w *= fo;
+                for (int x = 0; x < ATT_HEADS / W; x++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (ml[j].y != 0.0f) {
-                        const float f = mn == -INFINITY ? 1.0f : exp2_fast(ml[j].x - mn);
-                        lt = fmaf(f, ml[j].y, lt);
-                        s.x = fmaf(f, v[j].x, s.x);
-                        s.y = fmaf(f, v[j].y, s.y);
-                        s.z = fmaf(f, v[j].z, s.z);
-                        s.w = fmaf(f, v[j].w, s.w);
+                    for (int y = 0; y < 2; y++)
+                        ml[x][y] = warp + W * x < p.heads && lane + 32 * y < p.parts
+                                       ? __ldcg(reinterpret_cast<const float2 *>(part_of(lane + 32 * y) +
+                                                                                 (warp + W * x) * (HSP + 4) + HSP))
+                                       : make_float2(-INFINITY, 0.0f);
+            }
+            for (int j = warp; j < nj; j += W) {
+                const uint8_t *src = reinterpret_cast<const uint8_t *>(part_of(j0 + j)) + 16 * lane;
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(smem) + j * bytes + 16 * lane;
+#pragma unroll 4
+                for (int x = 0; x < bytes; x += 512)
+                    if (x + 16 * lane < bytes)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x), "l"(src + x) : "memory");
+            }
+            if (j0 == 0) {
+                // the heads' maxima and weights over all parts, meanwhile
+#pragma unroll
+                for (int x = 0; x < ATT_HEADS / W; x++) {
+                    const int h = warp + W * x;
+                    if (h >= p.heads) break;
+                    float mt = -INFINITY, lt = 0.0f;
+                    auto take = [&](float2 v) {
+                        if (v.y != 0.0f) {
+                            const float mn = fmaxf(mt, v.x);
+                            lt = lt * (mn == -INFINITY ? 1.0f : exp2_fast(mt - mn)) +
+                                 v.y * (mn == -INFINITY ? 1.0f : exp2_fast(v.x - mn));
+                            mt = mn;
+                        }
+                    };
+                    take(ml[x][0]);
+                    take(ml[x][1]);
+                    for (int j = lane + 64; j < p.parts; j += 32)
+                        take(__ldcg(reinterpret_cast<const float2 *>(part_of(j) + h * (HSP + 4) + HSP)));
+                    float top = mt;
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                    lt *= top == -INFINITY ? 1.0f : exp2_fast(mt - top);
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(0xFFFFFFFFu, lt, o);
+                    if (lane == 0) {
+                        wm[0][h] = top;
+                        wl[0][h] = lt;
                     }
                 }
             }
-            const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
-            *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < JT; c++) {
+                const int i = tid + 32 * W * c, h = i / F4, d = 4 * (i - h * F4);
+                if (h >= p.heads) break;
+                const float top = wm[0][h];
+                const float *ph = reinterpret_cast<const float *>(smem) + h * (HSP + 4);
+#pragma unroll 4
+                for (int j = 0; j < nj; j++, ph += bytes / 4) {
+                    const float2 ml = *reinterpret_cast<const float2 *>(ph + HSP);
+                    const float4 v = *reinterpret_cast<const float4 *>(ph + d);
+                    const float f = ml.y == 0.0f ? 0.0f : top == -INFINITY ? 1.0f : exp2_fast(ml.x - top);
+                    s[c].x = fmaf(f, v.x, s[c].x);
+                    s[c].y = fmaf(f, v.y, s[c].y);
+                    s[c].z = fmaf(f, v.z, s[c].z);
+                    s[c].w = fmaf(f, v.w, s[c].w);
+                }
+            }
         }
+#pragma unroll
+        for (int c = 0; c < JT; c++) {
+            const int i = tid + 32 * W * c, h = i / F4, d = 4 * (i - h * F4);
+            if (h >= p.heads) break;
+            const float lt = wl[0][h], inv = lt != 0.0f ? 1.0f / lt : 0.0f;
+            *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s[c].x * inv, s[c].y * inv, s[c].z * inv, s[c].w * inv);
+        }
+        __syncthreads();  // wm and wl are read
     }
 }
+
 }  // namespace kvp
 }  // namespace pk
 
@@ -1026,6 +1096,7 @@ static const char *shape_fault(KvPagedShape &s)
         if (st[i] > big) return "Page, token or head stride too large.";
         below += st[i] * (cnt[i] - 1);
     }
+    if (below / unit >= (uint64_t)1 << 32) return "A pool must be smaller than 64 GB.";
     return nullptr;
 }
 
@@ -1103,6 +1174,10 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
     kv->c.page_stride = s.page_stride;
     kv->c.token_stride = s.token_stride;
     kv->c.head_stride = s.head_stride;
+    const uint64_t unit = s.type == 1 ? 8 : 4;
+    kv->c.page_units = (uint32_t)(s.page_stride / unit);
+    kv->c.token_units = (uint32_t)(s.token_stride / unit);
+    kv->c.head_units = (uint32_t)(s.head_stride / unit);
     if (device < 0) return kv;
     int count = 0;
     cudaError_t e = cudaGetDeviceCount(&count);

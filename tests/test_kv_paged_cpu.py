@@ -58,6 +58,7 @@ def test_shape_layout(tmp_path):
     (dict(strides=(16 * 128, 120, 64)), "overlap"),
     (dict(strides=(16 * 128 - 8, 128, 64)), "overlap"),
     (dict(strides=(16 * 128, 128, 0)), "overlap"),
+    (dict(strides=(1 << 33, 128, 64)), "64 GB"),
     (dict(device=-2), "Invalid device"),
 ])
 def test_shapes_refused(change, why):
@@ -66,7 +67,7 @@ def test_shapes_refused(change, why):
 
 
 @pytest.mark.parametrize("strides", [(0, 0, 0), (16 * 128, 128, 64), (16 * 128, 64, 16 * 64), (128, 128 * 10, 64),
-                                     (4096, 136, 64), (1 << 33, 128, 64)])
+                                     (4096, 136, 64), (1 << 31, 128, 64)])
 def test_shapes_taken(strides):
     handle(strides=strides).close()
 
