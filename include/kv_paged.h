@@ -50,7 +50,7 @@ typedef struct {
     int page_tokens;     /* tokens of a page, any number >= 1 */
     int n_pages;         /* pages of a pool; n_pages * page_tokens < 2^31 */
     int max_requests;    /* rows of the block table, 1 .. KV_PAGED_MAX_REQUESTS */
-    int max_blocks;      /* entries of a row of the block table */
+    int max_blocks;      /* entries of a row of the block table; at most 2^30 tokens */
     /* Entries from a page, token or KV head to the next, multiples of 16
      * bytes; all 0: [page][token][KV head][channel] without gaps. Channels
      * are adjacent. */
@@ -81,6 +81,8 @@ const char *kv_paged_last_error(const KvPaged *kv);
 #define KV_PAGED_BAD_ROW 16    /* append: a slot past the pool or a position past the rotary table (row
                                   passed over); attend: a request past the table (row passed over) or a
                                   position past its row (its tokens end at the row's last) */
+#define KV_PAGED_TOO_MUCH 32   /* attend: rows x KV heads x tokens past what one call takes (16 TB of cache):
+                                  no output was written */
 int kv_paged_error(KvPaged *kv);
 
 /*

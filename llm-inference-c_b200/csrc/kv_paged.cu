@@ -306,27 +306,35 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
 // mma takes its operands straight from the registers that the softmax leaves
 // them in.
 //
-// Every warp of a CTA runs a ring of its own: STAGES tiles of TILE tokens
-// (keys and values, about 9 KB) are in flight by 16-byte async copies, with
-// the page numbers of the tile after them; a warp waits for no other before
-// an item's end. Tokens that a row may not see are zero-filled, never read.
-constexpr int ATT_WARPS = 4, ATT_HEADS = 8;
+// All items' tokens, cut into chunks, are shared out evenly over all resident
+// CTAs, whatever the rows' lengths. A warp takes every WARPS-th tile of a
+// chunk and waits for no other before an item's end: its ring of STAGES tiles
+// (keys and values, about 9 KB each) is filled by 16-byte async copies over
+// the ends of items, and the pages of the tile after them are looked up
+// meanwhile. Items that lie in one CTA's share are written at once; of the
+// others each CTA leaves its part in the scratch, and the last to arrive
+// joins them, in their order. Tokens that a row may not see are zero-filled,
+// never read.
+constexpr int ATT_HEADS = 8;
+constexpr float ATT_JOIN = 0.2f;  // the cost of a part over that of a chunk
 
 template <typename KV, int HSP>
 struct Geo {
     static constexpr bool HALF = sizeof(KV) == 2;
     static constexpr int TILE = HALF ? (HSP == 64 ? 32 : 16) : (HSP == 64 ? 16 : 8);  // tokens
-    static constexpr int CHUNK = ATT_WARPS * TILE;   // tokens: the unit in which work is shared out
+    static constexpr int WARPS = 4;
+    static constexpr int STAGES = HSP == 256 ? 1 : 2;
+    static constexpr int CTAS = HSP == 256 ? 2 : 3;  // per SM, as shared memory allows
+    static constexpr int CHUNK = WARPS * TILE;       // tokens: the unit in which work is shared out
     static constexpr int ROW = HSP * (int)sizeof(KV) + 16;  // bytes; 16 past a multiple of 128: no bank conflicts
     static constexpr int STAGE = 2 * TILE * ROW;
-    static constexpr int STAGES = HSP == 256 ? 3 : 2;
-    static constexpr int CTAS = HSP == 256 ? 1 : 3;  // per SM, as shared memory allows
     static constexpr int RING = STAGES * STAGE;
     static constexpr int SEGS = HSP * (int)sizeof(KV) / 16;  // 16-byte pieces of a token's head
-    static constexpr int QFRAG = (HALF ? HSP / 16 : HSP / 8) * 512;
-    static constexpr int SMEM = ATT_WARPS * RING + QFRAG;
-    static constexpr int OROW = HSP + 8;  // floats from a head to the next where warps leave their sums
-    static_assert(ATT_HEADS * OROW * 4 <= STAGE, "a warp's sums fit a stage");
+    static constexpr int KS = HALF ? HSP / 16 : HSP / 8;     // steps of a score's product
+    static constexpr int SMEM = WARPS * RING + KS * 512;     // rings, then q as the products' left operand
+    static constexpr int OROW = HSP + 8;                     // floats from a head to the next of sums that wait to be joined
+    static constexpr int PART = ATT_HEADS * OROW;            // floats of a part
+    static_assert(PART * 4 <= STAGE, "a warp's sums fit a stage");
 };
 
 struct AttendArgs {
@@ -339,7 +347,7 @@ struct AttendArgs {
     float *out;
     uint64_t q_stride;
     Cache c;
-    float *part;        // [2 * grid][ATT_HEADS][HSP + 4]: sums, then maximum and weight
+    float *part;        // [2 * grid][ATT_HEADS][OROW]: a head's sums, then its maximum and weight at HSP
     unsigned *arrived;  // [grid]: parts of the item that begins in CTA b and ends in another; wraps to 0 by itself
     int *err;
 };
@@ -394,7 +402,6 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
-
 // o = o f + the sum of both halves of a tile's product. The running sums are
 // kept outside the tensor cores, whose accumulators cut bits off instead of
 // rounding: over a thousand tokens that adds up to 2e-6 of the result, always
@@ -403,6 +410,11 @@ __device__ __forceinline__ void add_tile(float (&o)[2], const float (&x)[4], flo
 {
     o[0] = fmaf(o[0], f, x[0] + x[2]);
     o[1] = fmaf(o[1], f, x[1] + x[3]);
+}
+// 2^(x - top), for a part's maximum x and the maximum of all parts.
+__device__ __forceinline__ float weight_of(float x, float top)
+{
+    return top == -INFINITY ? 1.0f : exp2_fast(x - top);
 }
 
 // The visible tokens of a row of request `req` at position `last`, -1 for a
@@ -422,17 +434,21 @@ __device__ __forceinline__ int row_tokens(const AttendArgs &a, int req, int last
     return last + 1;
 }
 
-__host__ __device__ __forceinline__ int chunks_of(int tokens, int chunk)
+// Units of a row's items: its chunks, and one for the item's end, which costs
+// about as much.
+template <int CHUNK>
+__device__ __forceinline__ int units_of(int tokens)
 {
-    return tokens < 0 ? 0 : tokens == 0 ? 1 : (tokens - 1) / chunk + 1;
+    return tokens < 0 ? 0 : (int)(((unsigned)tokens + CHUNK - 1) / CHUNK) + 1;
 }
 
-// A place in a CTA's share of the work: chunk `c` of item `it` of row r. The
+// A place in a CTA's share of the work: unit c of item `it` of row r. The
 // next row's numbers are loaded a row ahead.
+template <int CHUNK>
 struct Place {
     int r, it, tokens, req, c;
     int next_req, next_pos;
-    long long left;  // chunks of the CTA's share from here on
+    int left;  // units of the share from here on
 
     __device__ __forceinline__ void ahead(const AttendArgs &a)
     {
@@ -441,16 +457,14 @@ struct Place {
             next_pos = a.row_pos[r + 1];
         }
     }
-    // chunks of this item in the share
-    __device__ __forceinline__ int span(int chunk) const
-    {
-        const int k = chunks_of(tokens, chunk) - c;
-        return left < k ? (int)left : k;
-    }
+    // units of this item in the share
+    __device__ __forceinline__ int span() const { return min(left, units_of<CHUNK>(tokens) - c); }
+    // the share's tokens of this item end before this one
+    __device__ __forceinline__ int stop() const { return min((long long)tokens, (long long)(c + span()) * CHUNK); }
     // on to the next item; the share has one more when left > 0
-    __device__ __forceinline__ void next(const AttendArgs &a, int chunk, int items)
+    __device__ __forceinline__ void next(const AttendArgs &a, int items)
     {
-        left -= span(chunk);
+        left -= span();
         c = 0;
         if (++it < items || left <= 0) return;
         it = 0;
@@ -473,81 +487,93 @@ struct Part {
 };
 
 template <typename KV, int HSP>
-__global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_kernel(const AttendArgs a)
+__global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) attend_kernel(const AttendArgs a)
 {
     using G = Geo<KV, HSP>;
-    constexpr int TILE = G::TILE, CHUNK = G::CHUNK, W = ATT_WARPS, NT = TILE / 8, DT = HSP / 8;
-    constexpr int JT = ATT_HEADS * HSP / 4 / (32 * W);  // pieces of 4 channels of all heads, per thread
-    extern __shared__ __align__(16) uint8_t smem[];  // rings, then q
-    __shared__ float row_unit[ATT_HEADS];            // score = product * row_unit
-    __shared__ float wm[W][ATT_HEADS], wl[W][ATT_HEADS];
-    __shared__ const float *wo[W];                   // where warp w left its sums (NULL: it had no tiles)
-    __shared__ uint32_t masks[W][G::STAGES];
-    __shared__ long long sums[W];
-    __shared__ int tops[W];
-    __shared__ Place begin;
+    constexpr int TILE = G::TILE, CHUNK = G::CHUNK, W = G::WARPS, NT = TILE / 8, DT = HSP / 8, KS = G::KS;
+    constexpr int JT = (ATT_HEADS * HSP / 4 + 32 * W - 1) / (32 * W);  // pieces of 4 channels of all heads, per thread
+    constexpr int HW = (ATT_HEADS + W - 1) / W;  // heads of a warp
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float head_unit[ATT_HEADS];           // score = product * unit
+    __shared__ float wm[ATT_HEADS][W], wl[ATT_HEADS][W];  // warps' maxima and weights
+    __shared__ const float *wo[W];                   // where a warp left its sums
+    __shared__ uint32_t masks[W][G::STAGES];         // the tokens of the ring's tiles that count
+    __shared__ uint4 sums[W];  // warps' units, 256ths of units, longest items
+    __shared__ Place<CHUNK> begin;
     __shared__ Part pend[2];  // the share's first item, begun by another CTA, and its last, ended by another
     __shared__ int is_last[2];
+    __shared__ float jm[ATT_HEADS], jl[ATT_HEADS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     const int items = a.kv_heads * a.groups, b = blockIdx.x;
+    const int group = a.heads / a.kv_heads, F4 = a.hs >> 2;
+    auto heads_of = [&](int it, int &h0, int &H) {
+        const int kvh = it / a.groups, grp = it - kvh * a.groups;
+        h0 = kvh * group + grp * a.group_heads;
+        H = min(a.group_heads, group - grp * a.group_heads);
+    };
 
-    // This CTA's share: all rows' chunks, in rows' and items' order, are cut
-    // into equal shares. Every CTA adds the chunks up for itself.
+    // ---- shares: every CTA adds the units of all rows up for itself ----
+    // (2^31 units, 64 TB of cache, are refused)
     const int each = (a.n + 32 * W - 1) / (32 * W), r0 = min(a.n, tid * each), r1 = min(a.n, r0 + each);
     int fault = 0;
     long long mine = 0;
-    int req0 = -1, tokens0 = -1;  // this thread's first row
     int longest = 0;
     for (int r = r0; r < r1; r++) {
-        const int req = a.row_request[r], tokens = row_tokens(a, req, a.row_pos[r], fault);
-        mine += (long long)chunks_of(tokens, CHUNK) * items;
-        longest = max(longest, chunks_of(tokens, CHUNK));
-        if (r == r0) {
-            req0 = req;
-            tokens0 = tokens;
-        }
+        const int req = a.row_request[r], tokens = row_tokens(a, req, a.row_pos[r], fault), u = units_of<CHUNK>(tokens);
+        mine += (long long)u * items;
+        longest = max(longest, u);
     }
     if (fault && b == 0) atomicOr(a.err, fault);
-    long long before = mine;
+    // sums in 32 bits, and those of 256ths, which cannot overflow, beside them
+    const unsigned own = (unsigned)min(mine, 1ll << 31);
+    unsigned before = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xFFFFFFFFu, before, o);
+        const unsigned u = __shfl_up_sync(0xFFFFFFFFu, before, o);
         if (lane >= o) before += u;
     }
+    const unsigned rough = __reduce_add_sync(0xFFFFFFFFu, own >> 8);
     longest = __reduce_max_sync(0xFFFFFFFFu, longest);
-    if (lane == 31) {
-        sums[warp] = before;
-        tops[warp] = longest;
-    }
+    if (lane == 31) sums[warp] = make_uint4(before, rough, longest, 0);
+    if (tid < 2) pend[tid].parts = 0;
     __syncthreads();
-    long long all = 0;
-    before -= mine;
+    unsigned all = 0, much = 0;
+    before -= own;
+#pragma unroll
     for (int w = 0; w < W; w++) {
+        const uint4 x = sums[w];
         if (w == warp) before += all;
-        all += sums[w];
-        longest = max(longest, tops[w]);
+        all += x.x;
+        much += x.y;
+        longest = max(longest, (int)x.z);
     }
-    // A part costs the CTA that joins it about 0.25 us, a chunk in a GPU that
-    // is not full about 0.6 us, so where all CTAs together would have less,
-    // shares are not smaller than makes both sides equal for the longest item:
-    // c parts of longest / c chunks.
-    const long long share = max((all + gridDim.x - 1) / gridDim.x, (long long)__fsqrt_rn(0.4f * longest)), first = share * b;
+    if (much >= (1u << 23) - 32 * W) {
+        if (b == 0 && tid == 0) atomicOr(a.err, KV_PAGED_TOO_MUCH);
+        return;
+    }
+    // A part costs the CTA that joins it about 0.2 us, a chunk in a GPU that
+    // is not full about 1 us: where that leaves less to all CTAs, shares are
+    // not smaller than makes both sides equal for the longest item, whose
+    // parts are longest / share, nor than a chunk and an item's end.
+    const unsigned even = (all + gridDim.x - 1) / gridDim.x;
+    const unsigned share = max(max(even, 2u), (unsigned)__fsqrt_rn(ATT_JOIN * longest));
+    const unsigned first = (unsigned)min((unsigned long long)share * b, 1ull << 31);
     if (first >= all) return;
-    if (first >= before && first < before + mine) {
-        long long at = before;
+    if (first - before < own) {
+        unsigned at = before;
         for (int r = r0; r < r1; r++) {
-            const int req = r == r0 ? req0 : a.row_request[r];
-            const int tokens = r == r0 ? tokens0 : row_tokens(a, req, a.row_pos[r], fault), ch = chunks_of(tokens, CHUNK);
-            if (first < at + (long long)ch * items) {
+            const int req = a.row_request[r], tokens = row_tokens(a, req, a.row_pos[r], fault);
+            const unsigned u = units_of<CHUNK>(tokens);
+            if (first - at < u * items) {
                 begin.r = r;
                 begin.req = req;
                 begin.tokens = tokens;
-                begin.it = (int)((first - at) / ch);
-                begin.c = (int)((first - at) % ch);
-                begin.left = min(share, all - first);
+                begin.it = (int)((first - at) / u);
+                begin.c = (int)((first - at) - begin.it * u);
+                begin.left = (int)min(share, all - first);
                 break;
             }
-            at += (long long)ch * items;
+            at += u * items;
         }
     }
     __syncthreads();
@@ -558,17 +584,16 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
     const int segs = a.hs * (int)sizeof(KV) / 16;
 
     // ---- loads: tile after tile of this warp, over the items' ends ----
-    Place lp = begin;
+    Place<CHUNK> lp = begin;
     lp.ahead(a);
-    int lt = warp, l_end = 0, l_tok0 = 0;  // tile of the item in the share, tiles, first token
-    int l_stop = 0;                        // the tokens end here
+    Place<CHUNK> cp = lp;
+    int l_tok = 0, l_stop = 0;  // the next tile's first token, and the share's end of the item
     const int *l_table = nullptr;
     uint32_t l_head = 0;
     bool l_more = true;
     auto open_item = [&]() {
-        l_tok0 = lp.c * CHUNK;
-        l_stop = min(lp.tokens, (lp.c + lp.span(CHUNK)) * CHUNK);
-        l_end = l_stop > l_tok0 ? (l_stop - l_tok0 + TILE - 1) / TILE : 0;
+        l_tok = lp.c * CHUNK + warp * TILE;
+        l_stop = lp.stop();
         l_table = a.table + (size_t)lp.req * a.c.max_blocks;
         l_head = (uint32_t)(lp.it / a.groups) * a.c.head_units;
     };
@@ -577,20 +602,18 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
     int nx_page = -1, nx_place = 0;
     // looks up the pages of the next tile: token `lane` of it
     auto look = [&]() {
-        while (l_more && lt >= l_end) {
-            lp.next(a, CHUNK, items);
+        while (l_more && l_tok >= l_stop) {
+            lp.next(a, items);
             if (lp.left <= 0) {
                 l_more = false;
             } else {
-                lt = warp;
                 open_item();
             }
         }
         nx_any = l_more;
-        nx_page = -1;
         nx_ok = false;
         if (!l_more) return;
-        const int tok = l_tok0 + lt * TILE + lane;
+        const int tok = l_tok + lane;
         if (lane < TILE && tok < l_stop) {
             const int blk = div_by(a.c.page, tok);
             nx_place = tok - blk * (int)a.c.page.d;
@@ -598,26 +621,29 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
             nx_ok = true;
         }
         nx_at = l_head;
-        lt += W;
+        l_tok += CHUNK;
     };
     auto issue = [&](int slot) {
         if (nx_any) {
             uint32_t at = nx_at;
-            if (nx_ok && (nx_page < 0 || nx_page >= a.c.n_pages)) {
+            const int page = nx_page, place = nx_place;
+            bool ok = nx_ok;
+            look();  // the tile after this one: its page numbers are there when it is issued
+            if (ok && (page < 0 || page >= a.c.n_pages)) {
                 atomicOr(a.err, KV_PAGED_BAD_PAGE);
-                nx_ok = false;
+                ok = false;
             }
-            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, nx_ok);
-            if (nx_ok) at += (uint32_t)nx_page * a.c.page_units + (uint32_t)nx_place * a.c.token_units;
+            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok);
             if (lane == 0) masks[warp][slot] = mask;
+            if (ok) at += (uint32_t)page * a.c.page_units + (uint32_t)place * a.c.token_units;
             const uint32_t dst0 = ring_s + slot * G::STAGE;
 #pragma unroll
             for (int i = 0; i < TILE * G::SEGS / 32; i++) {
                 const int idx = lane + 32 * i, key = idx / G::SEGS, seg = idx % G::SEGS;
                 const uint32_t from = __shfl_sync(0xFFFFFFFFu, at, key);
-                const bool ok = ((mask >> key) & 1u) && seg < segs;
-                const int bytes = ok ? 16 : 0;
-                const uint64_t e = ok ? (uint64_t)(from + seg) * 16 : 0;
+                const bool in = ((mask >> key) & 1u) && seg < segs;
+                const int bytes = in ? 16 : 0;
+                const uint64_t e = in ? (uint64_t)(from + seg) * 16 : 0;
                 const uint32_t dst = dst0 + key * G::ROW + seg * 16;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
                              "l"(static_cast<const uint8_t *>(a.k_pool) + e), "r"(bytes)
@@ -628,21 +654,15 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (nx_any) look();
     };
-    // ---- q: head h of an item by warp h mod W; loaded an item ahead ----
-    float2 qn[ATT_HEADS / W][HSP / 64];
-    const int group = a.heads / a.kv_heads;
-    auto heads_of = [&](const Place &p, int &h0, int &H) {
-        const int kvh = p.it / a.groups, grp = p.it - kvh * a.groups;
-        h0 = kvh * group + grp * a.group_heads;
-        H = min(a.group_heads, group - grp * a.group_heads);
-    };
-    auto load_q = [&](const Place &p) {
+
+    // ---- q: head h by warp h mod W; loaded an item ahead ----
+    float2 qn[HW][HSP / 64];
+    auto ask_q = [&](const Place<CHUNK> &p) {
         int h0, H;
-        heads_of(p, h0, H);
+        heads_of(p.it, h0, H);
 #pragma unroll
-        for (int k = 0; k < ATT_HEADS / W; k++) {
+        for (int k = 0; k < HW; k++) {
             const int h = warp + k * W;
             const float *q = a.q + (size_t)p.r * a.q_stride + (size_t)(h0 + h) * a.hs;
 #pragma unroll
@@ -652,11 +672,13 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
             }
         }
     };
-    auto store_q = [&]() {
+    // q as the left operand: row g is head g's, row g + 8 its lower parts
+    auto make_q = [&]() {
         const float cq = a.scale * 1.44269504088896f;  // scores in base 2
 #pragma unroll
-        for (int k = 0; k < ATT_HEADS / W; k++) {
+        for (int k = 0; k < HW; k++) {
             const int h = warp + k * W;
+            if (h >= ATT_HEADS) break;
             float x[HSP / 32];
             float big = 0.0f;
 #pragma unroll
@@ -678,7 +700,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
 #pragma unroll
                 for (int i = 0; i < HSP / 32; i++) x[i] *= f;
             }
-            if (lane == 0) row_unit[h] = unit;
+            if (lane == 0) head_unit[h] = unit;
 #pragma unroll
             for (int i = 0; i < HSP / 64; i++) {
                 const int d = 2 * lane + 64 * i;
@@ -701,32 +723,52 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
             }
         }
     };
+    auto q_step = [&](int k, uint32_t (&qa)[4]) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(qf + k * 128 + lane * 4);
+        qa[0] = v.x;
+        qa[1] = v.y;
+        qa[2] = v.z;
+        qa[3] = v.w;
+    };
 
-    // ---- items ----
-    Place cp = lp;
-    int slot = 0;
-    if (tid < 2) pend[tid].parts = 0;
-    load_q(cp);  // ahead of the tiles: behind them it would wait for all that all CTAs ask for
+    // ---- items of the share: one loop, so that each part of it is there once
+    // (instructions that a warp meets for the first time cost it a fetch) ----
+    ask_q(cp);  // ahead of the tiles: behind them it would wait for what all CTAs ask for
     open_item();
     look();
+    int slot = 0, fill = G::STAGES;  // tiles to ask for before the next is used
+    int tok = cp.c * CHUNK + warp * TILE, stop = cp.stop();
+    bool hold = false;  // this warp's last slot waits for the item's end
+    bool fresh = true, used = false;  // q is to be made; this warp has had a tile of the item
+    float o[DT][2], m = -INFINITY, l = 0.0f, unit = 1.0f;
 #pragma unroll
-    for (int s = 0; s < G::STAGES; s++) issue(s);
-    store_q();
-    __syncthreads();
+    for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
+    if (tid < 2) pend[tid].parts = 0;
+    Place<CHUNK> np = cp;
     while (true) {
-        const int span = cp.span(CHUNK), tok0 = cp.c * CHUNK, stop = min(cp.tokens, (cp.c + span) * CHUNK);
-        const int tiles = stop > tok0 ? (stop - tok0 + TILE - 1) / TILE : 0;
-        int h0, H;
-        heads_of(cp, h0, H);
-        Place np = cp;
-        np.next(a, CHUNK, items);
-        if (np.left > 0) load_q(np);
-        const float unit = row_unit[g];
-        float o[DT][2], m = -INFINITY, l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
-        int hold = -1;  // the slot of this warp's last tile, refilled after the item's end
-        for (int tile = warp; tile < tiles; tile += W) {
+        if (fill > 0) {
+            issue(slot);
+            slot = slot + 1 == G::STAGES ? 0 : slot + 1;
+            fill--;
+            continue;
+        }
+        if (fresh) {
+            // the first item's q; a later one's is made where the item before it ends
+            if (cp.left == begin.left) make_q();
+            __syncthreads();  // q is there, and the sums of the item before are read
+            unit = head_unit[g];
+            np.next(a, items);
+            if (np.left > 0) ask_q(np);
+            fresh = false;
+            if (hold) {
+                hold = false;
+                fill = 1;
+                continue;
+            }
+        }
+        if (tok < stop) {
+            tok += CHUNK;
+            used = true;
             asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 1) : "memory");
             __syncwarp();
             const uint32_t mask = masks[warp][slot];
@@ -738,9 +780,9 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
                 if (G::HALF) {
                     const uint32_t at = ks_s + ((lane >> 4) * 8 + (lane & 7)) * G::ROW + ((lane >> 3) & 1) * 16;
 #pragma unroll
-                    for (int ks = 0; ks < HSP / 16; ks++) {
-                        const uint4 qv = *reinterpret_cast<const uint4 *>(qf + ks * 128 + lane * 4);
-                        const uint32_t qa[4] = {qv.x, qv.y, qv.z, qv.w};
+                    for (int ks = 0; ks < KS; ks++) {
+                        uint32_t qa[4];
+                        q_step(ks, qa);
 #pragma unroll
                         for (int j = 0; j < NT / 2; j++) {
                             uint32_t kb[4];
@@ -755,10 +797,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
                     for (int j = 0; j < NT; j++) s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.0f;
                     const uint32_t at = ks_s + (lane & 7) * G::ROW + (lane >> 3) * 16;
 #pragma unroll
-                    for (int ks = 0; ks < HSP / 16; ks++) {
-                        const uint4 q0 = *reinterpret_cast<const uint4 *>(qf + 2 * ks * 128 + lane * 4);
-                        const uint4 q1 = *reinterpret_cast<const uint4 *>(qf + (2 * ks + 1) * 128 + lane * 4);
-                        const uint32_t qa[4] = {q0.x, q0.y, q0.z, q0.w}, qb[4] = {q1.x, q1.y, q1.z, q1.w};
+                    for (int ks = 0; ks < KS / 2; ks++) {
+                        uint32_t qa[4], qb[4];
+                        q_step(2 * ks, qa);
+                        q_step(2 * ks + 1, qb);
 #pragma unroll
                         for (int j = 0; j < NT; j++) {
                             uint32_t kb[4], hi[4], lo[4];
@@ -789,7 +831,7 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.0f : exp2_fast(m - mn);
+                const float mn = fmaxf(m, top), f = weight_of(m, mn);
                 m = mn;
                 l *= f;
                 // 2^12 p in a half cache's products: its parts' smallest
@@ -851,85 +893,89 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
                 }
             }
             __syncwarp();
-            if (tile + W < tiles) {
-                issue(slot);
-            } else {
-                hold = slot;
+            if (tok < stop) {
+                fill = 1;
+                continue;
             }
-            slot = slot + 1 == G::STAGES ? 0 : slot + 1;
+            hold = true;  // the last tile's slot is filled again after the item's end
         }
-        // the warps' sums, each in the slot of its last tile
+        // ---- the item's end: the warps' sums, each in the slot of its last tile ----
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-        if (hold >= 0) {
-            float *dst = reinterpret_cast<float *>(ring + hold * G::STAGE) + g * G::OROW;
+        float *mine_o = reinterpret_cast<float *>(ring + slot * G::STAGE);
+        if (used) {
+            float *dst = mine_o + g * G::OROW;
 #pragma unroll
-            for (int i = 0; i < DT; i++) {
-                const float x = o[i][0], y = o[i][1];
+            for (int i = 0; i < DT; i += G::HALF ? 1 : 4) {
                 if (G::HALF) {
-                    *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t4) = make_float2(x, y);
+                    *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t4) = make_float2(o[i][0], o[i][1]);
                 } else {
-                    dst[32 * (i / 4) + 8 * t4 + (i & 3)] = x;
-                    dst[32 * (i / 4) + 8 * t4 + 4 + (i & 3)] = y;
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        *reinterpret_cast<float4 *>(dst + 8 * i + 8 * t4 + 4 * j) =
+                            make_float4(o[i][j], o[i + (G::HALF ? 0 : 1)][j], o[i + (G::HALF ? 0 : 2)][j],
+                                        o[i + (G::HALF ? 0 : 3)][j]);
                 }
             }
         }
         if (t4 == 0) {
-            wm[warp][g] = m;
-            wl[warp][g] = hold >= 0 ? l : 0.0f;
+            wm[g][warp] = m;
+            wl[g][warp] = used ? l : 0.0f;
         }
-        if (lane == 0) wo[warp] = hold >= 0 ? reinterpret_cast<const float *>(ring + hold * G::STAGE) : nullptr;
+        if (lane == 0) wo[warp] = mine_o;
         __syncthreads();
-        if (np.left > 0) store_q();  // every warp is done with this item's
-        const int ch = chunks_of(cp.tokens, CHUNK);
-        const bool whole = cp.c == 0 && span == ch;
-        const int F4 = a.hs >> 2;
+        if (np.left > 0) make_q();  // every warp is done with this item's
+        const int units = units_of<CHUNK>(cp.tokens);
+        const bool whole = cp.c == 0 && cp.span() == units;
         const int side = cp.c == 0 ? 1 : 0;
-        float *part = a.part + (size_t)(2 * b + side) * ATT_HEADS * (HSP + 4);
+        int h0, H;
+        heads_of(cp.it, h0, H);
+        float *part = a.part + (size_t)(2 * b + side) * G::PART;
         float *out = a.out + ((size_t)cp.r * a.heads + h0) * a.hs;
         for (int i = tid; i < H * F4; i += 32 * W) {
             const int h = i / F4, d = 4 * (i - h * F4);
             float mt = -INFINITY, lt = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; w++)
-                if (wl[w][h] != 0.0f) mt = fmaxf(mt, wm[w][h]);
+                if (wl[h][w] != 0.0f) mt = fmaxf(mt, wm[h][w]);
             float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                if (wl[w][h] != 0.0f) {
-                    const float f = mt == -INFINITY ? 1.0f : exp2_fast(wm[w][h] - mt);
+                if (wl[h][w] != 0.0f) {
+                    const float f = weight_of(wm[h][w], mt);
                     const float4 v = *reinterpret_cast<const float4 *>(wo[w] + h * G::OROW + d);
-                    lt = fmaf(f, wl[w][h], lt);
+                    lt = fmaf(f, wl[h][w], lt);
                     s.x = fmaf(f, v.x, s.x);
                     s.y = fmaf(f, v.y, s.y);
                     s.z = fmaf(f, v.z, s.z);
                     s.w = fmaf(f, v.w, s.w);
                 }
             }
-            if (whole) {
-                const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
-                *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
-            } else {
-                float *ph = part + (size_t)h * (HSP + 4);
-                *reinterpret_cast<float4 *>(ph + d) = s;
-                if (d == 0) *reinterpret_cast<float2 *>(ph + HSP) = make_float2(mt, lt);
-            }
+            const float inv = !whole ? 1.0f : lt != 0.0f ? 1.0f / lt : 0.0f;
+            float *dst = whole ? out + h * a.hs : part + h * G::OROW;
+            *reinterpret_cast<float4 *>(dst + d) = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+            if (!whole && d == 0) *reinterpret_cast<float2 *>(dst + HSP) = make_float2(mt, lt);
         }
         if (!whole && tid == 0) {
-            // the item's chunks begin at `item0` of all rows' chunks
-            const long long item0 = first + (min(share, all - first) - cp.left) - cp.c;
-            const int b0 = (int)(item0 / share);
+            // the item's units begin at `start` of all items' units
+            const unsigned start = first + (begin.left - cp.left) - cp.c;
             Part &p = pend[side];
             p.r = cp.r;
             p.h0 = h0;
             p.heads = H;
-            p.b0 = b0;
-            p.parts = (int)((item0 + ch - 1) / share) - b0 + 1;
+            p.b0 = side == 1 ? b : (int)(start / share);
+            p.parts = (int)((start + units - 1) / share) - p.b0 + 1;
         }
-        if (np.left <= 0) break;
         cp = np;
-        __syncthreads();  // the sums are read: their slots may be filled; q is there
-        if (hold >= 0) issue(hold);
+        if (cp.left <= 0) break;
+        tok = cp.c * CHUNK + warp * TILE;
+        stop = cp.stop();
+        fresh = true;
+        used = false;
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 
@@ -941,17 +987,17 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
     if (tid < 2) {
         const Part p = pend[tid];
         is_last[tid] = p.parts > 0 && atomicInc(a.arrived + p.b0, (unsigned)p.parts - 1) == (unsigned)p.parts - 1;
+        __threadfence();
     }
     __syncthreads();
     for (int k = 0; k < 2; k++) {
         if (!is_last[k]) continue;
-        __threadfence();
         const Part p = pend[k];
-        const int F4 = a.hs >> 2, bytes = p.heads * (HSP + 4) * 4, fit = W * G::RING / bytes;
+        const int bytes = p.heads * G::OROW * 4, fit = W * G::RING / bytes;
         float *out = a.out + ((size_t)p.r * a.heads + p.h0) * a.hs;
-        const float *src0 = a.part + (size_t)2 * p.b0 * ATT_HEADS * (HSP + 4);
+        const float *src0 = a.part + (size_t)2 * p.b0 * G::PART;
         // part j of the item: the first CTA's is its last item, the others' their first
-        auto part_of = [&](int j) { return src0 + (size_t)(2 * j + (j == 0 ? 1 : 0)) * ATT_HEADS * (HSP + 4); };
+        auto part_of = [&](int j) { return src0 + (size_t)(2 * j + (j == 0 ? 1 : 0)) * G::PART; };
         float4 s[JT];
 #pragma unroll
         for (int c = 0; c < JT; c++) s[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -959,17 +1005,6 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
             // as many parts as fit, all their loads in flight at once; a warp takes every W-th part
             const int nj = min(fit, p.parts - j0);
             __syncthreads();
-            float2 ml[ATT_HEADS / W][2];  // heads warp, warp + W: the first 64 parts' maxima and weights
-            if (j0 == 0) {
-#pragma unroll
-                for (int x = 0; x < ATT_HEADS / W; x++)
-#pragma unroll
-                    for (int y = 0; y < 2; y++)
-                        ml[x][y] = warp + W * x < p.heads && lane + 32 * y < p.parts
-                                       ? __ldcg(reinterpret_cast<const float2 *>(part_of(lane + 32 * y) +
-                                                                                 (warp + W * x) * (HSP + 4) + HSP))
-                                       : make_float2(-INFINITY, 0.0f);
-            }
             for (int j = warp; j < nj; j += W) {
                 const uint8_t *src = reinterpret_cast<const uint8_t *>(part_of(j0 + j)) + 16 * lane;
                 const uint32_t dst = (uint32_t)__cvta_generic_to_shared(smem) + j * bytes + 16 * lane;
@@ -978,35 +1013,26 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
                     if (x + 16 * lane < bytes)
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + x), "l"(src + x) : "memory");
             }
-            if (j0 == 0) {
-                // the heads' maxima and weights over all parts, meanwhile
-#pragma unroll
-                for (int x = 0; x < ATT_HEADS / W; x++) {
-                    const int h = warp + W * x;
-                    if (h >= p.heads) break;
-                    float mt = -INFINITY, lt = 0.0f;
-                    auto take = [&](float2 v) {
-                        if (v.y != 0.0f) {
-                            const float mn = fmaxf(mt, v.x);
-                            lt = lt * (mn == -INFINITY ? 1.0f : exp2_fast(mt - mn)) +
-                                 v.y * (mn == -INFINITY ? 1.0f : exp2_fast(v.x - mn));
-                            mt = mn;
-                        }
-                    };
-                    take(ml[x][0]);
-                    take(ml[x][1]);
-                    for (int j = lane + 64; j < p.parts; j += 32)
-                        take(__ldcg(reinterpret_cast<const float2 *>(part_of(j) + h * (HSP + 4) + HSP)));
-                    float top = mt;
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-                    lt *= top == -INFINITY ? 1.0f : exp2_fast(mt - top);
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(0xFFFFFFFFu, lt, o);
-                    if (lane == 0) {
-                        wm[0][h] = top;
-                        wl[0][h] = lt;
+            // the heads' maxima and weights over all parts, meanwhile
+            for (int h = warp; j0 == 0 && h < p.heads; h += W) {
+                float mt = -INFINITY, lt = 0.0f;
+                for (int j = lane; j < p.parts; j += 32) {
+                    const float2 v = __ldcg(reinterpret_cast<const float2 *>(part_of(j) + h * G::OROW + HSP));
+                    if (v.y != 0.0f) {
+                        const float mn = fmaxf(mt, v.x);
+                        lt = lt * weight_of(mt, mn) + v.y * weight_of(v.x, mn);
+                        mt = mn;
                     }
+                }
+                float top = mt;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+                lt *= weight_of(mt, top);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(0xFFFFFFFFu, lt, o);
+                if (lane == 0) {
+                    jm[h] = top;
+                    jl[h] = lt;
                 }
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
@@ -1015,13 +1041,13 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
             for (int c = 0; c < JT; c++) {
                 const int i = tid + 32 * W * c, h = i / F4, d = 4 * (i - h * F4);
                 if (h >= p.heads) break;
-                const float top = wm[0][h];
-                const float *ph = reinterpret_cast<const float *>(smem) + h * (HSP + 4);
+                const float top = jm[h];
+                const float *ph = reinterpret_cast<const float *>(smem) + h * G::OROW;
 #pragma unroll 4
                 for (int j = 0; j < nj; j++, ph += bytes / 4) {
-                    const float2 ml = *reinterpret_cast<const float2 *>(ph + HSP);
+                    const float2 v2 = *reinterpret_cast<const float2 *>(ph + HSP);
                     const float4 v = *reinterpret_cast<const float4 *>(ph + d);
-                    const float f = ml.y == 0.0f ? 0.0f : top == -INFINITY ? 1.0f : exp2_fast(ml.x - top);
+                    const float f = v2.y == 0.0f ? 0.0f : weight_of(v2.x, top);
                     s[c].x = fmaf(f, v.x, s[c].x);
                     s[c].y = fmaf(f, v.y, s[c].y);
                     s[c].z = fmaf(f, v.z, s[c].z);
@@ -1033,10 +1059,10 @@ __global__ void __launch_bounds__(32 * ATT_WARPS, Geo<KV, HSP>::CTAS) attend_ker
         for (int c = 0; c < JT; c++) {
             const int i = tid + 32 * W * c, h = i / F4, d = 4 * (i - h * F4);
             if (h >= p.heads) break;
-            const float lt = wl[0][h], inv = lt != 0.0f ? 1.0f / lt : 0.0f;
+            const float lt = jl[h], inv = lt != 0.0f ? 1.0f / lt : 0.0f;
             *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s[c].x * inv, s[c].y * inv, s[c].z * inv, s[c].w * inv);
         }
-        __syncthreads();  // wm and wl are read
+        __syncthreads();  // jm and jl are read
     }
 }
 
@@ -1055,7 +1081,7 @@ struct KvPaged {
     int *err;           // error bits
     unsigned *map_arrived;
     unsigned *arrived;  // attend: [grid]
-    float *part;        // attend: [2 * grid][ATT_HEADS][hsp + 4]
+    float *part;        // attend: CTAs' parts
     char msg[256];
 };
 
@@ -1069,8 +1095,8 @@ static const char *shape_fault(KvPagedShape &s)
         return "Pages and page size must be positive, with less than 2^31 tokens in all.";
     if (s.max_requests < 1 || s.max_requests > KV_PAGED_MAX_REQUESTS)
         return "The block table takes 1 to 4096 requests.";
-    if (s.max_blocks < 1 || (long long)s.max_blocks * s.page_tokens > 0x7FFFFFFFll)
-        return "A request's blocks must be positive, with less than 2^31 tokens in all.";
+    if (s.max_blocks < 1 || (long long)s.max_blocks * s.page_tokens > 1ll << 30)
+        return "A request's blocks must be positive, with at most 2^30 tokens in all.";
     const uint64_t hs = (uint64_t)s.head_size, unit = s.type == 1 ? 8 : 4, big = (uint64_t)1 << 40;
     if (s.page_stride == 0 && s.token_stride == 0 && s.head_stride == 0) {
         s.head_stride = hs;
@@ -1132,20 +1158,15 @@ static int launched(KvPaged *kv, const char *what)
     return 0;
 }
 
-// The attention kernel of a handle, its dynamic shared memory, and the call of
-// `use` with them.
+// use(kernel, threads, dynamic shared memory, floats of a part) of a handle's attention.
 template <typename F>
 static auto with_attend(const KvPaged *kv, F use)
 {
     using namespace kvp;
-    if (kv->s.type == 1) {
-        if (kv->hsp == 64) return use(attend_kernel<__half, 64>, Geo<__half, 64>::SMEM);
-        if (kv->hsp == 128) return use(attend_kernel<__half, 128>, Geo<__half, 128>::SMEM);
-        return use(attend_kernel<__half, 256>, Geo<__half, 256>::SMEM);
-    }
-    if (kv->hsp == 64) return use(attend_kernel<float, 64>, Geo<float, 64>::SMEM);
-    if (kv->hsp == 128) return use(attend_kernel<float, 128>, Geo<float, 128>::SMEM);
-    return use(attend_kernel<float, 256>, Geo<float, 256>::SMEM);
+#define KVP_CASE(KV, HSP) use(attend_kernel<KV, HSP>, 32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::SMEM, Geo<KV, HSP>::PART)
+    if (kv->s.type == 1) return kv->hsp == 64 ? KVP_CASE(__half, 64) : kv->hsp == 128 ? KVP_CASE(__half, 128) : KVP_CASE(__half, 256);
+    return kv->hsp == 64 ? KVP_CASE(float, 64) : kv->hsp == 128 ? KVP_CASE(float, 128) : KVP_CASE(float, 256);
+#undef KVP_CASE
 }
 
 static bool off16(const void *p)
@@ -1185,19 +1206,19 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
     if (e == cudaSuccess) {
         OnDevice on(device);
         e = on.ok ? cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device) : cudaErrorInvalidDevice;
+        size_t parts = 0;
         kv->hsp = s.head_size <= 64 ? 64 : s.head_size <= 128 ? 128 : 256;
         if (e == cudaSuccess) {
-            e = with_attend(kv, [&](auto kernel, int smem) {
+            e = with_attend(kv, [&](auto kernel, int threads, int smem, int floats) {
                 int per_sm = 0;
                 cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-                if (x == cudaSuccess)
-                    x = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, 32 * kvp::ATT_WARPS, smem);
+                if (x == cudaSuccess) x = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem);
                 kv->grid = per_sm * kv->sms;
+                parts = (size_t)kv->grid * 2 * floats * 4;
                 return x == cudaSuccess && per_sm < 1 ? cudaErrorInvalidConfiguration : x;
             });
         }
         const size_t flags = 256 + (((size_t)kv->grid * 4 + 255) & ~(size_t)255);
-        const size_t parts = (size_t)2 * kv->grid * kvp::ATT_HEADS * (kv->hsp + 4) * 4;
         if (e == cudaSuccess) e = cudaMalloc(&kv->scratch, flags + parts);
         if (e == cudaSuccess) e = cudaMemset(kv->scratch, 0, flags);
         if (e == cudaSuccess)
@@ -1352,9 +1373,9 @@ extern "C" int kv_paged_attend(KvPaged *kv, const float *q, const void *k_pool, 
     a.arrived = kv->arrived;
     a.err = kv->err;
     cudaGetLastError();
-    with_attend(kv, [&](auto kernel, int smem) {
-        kernel<<<kv->grid, 32 * kvp::ATT_WARPS, smem, (cudaStream_t)stream>>>(a);
-        return 0;
+    with_attend(kv, [&](auto kernel, int threads, int smem, int) {
+        kernel<<<kv->grid, threads, smem, (cudaStream_t)stream>>>(a);
+        return cudaSuccess;
     });
     return launched(kv, "attend");
 }
