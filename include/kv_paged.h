@@ -48,7 +48,7 @@ typedef struct {
     int head_size;       /* a multiple of 8, 8 .. 256 */
     uint32_t type;       /* GGML type id of the pools' entries: 0 F32 or 1 F16 */
     int page_tokens;     /* tokens of a page, any number >= 1 */
-    int n_pages;         /* pages of a pool; n_pages * page_tokens < 2^31 */
+    int n_pages;         /* pages of a pool; n_pages * page_tokens at most 2^30 */
     int max_requests;    /* rows of the block table, 1 .. KV_PAGED_MAX_REQUESTS */
     int max_blocks;      /* entries of a row of the block table; at most 2^30 tokens */
     /* Entries from a page, token or KV head to the next, multiples of 16

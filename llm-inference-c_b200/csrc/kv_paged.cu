@@ -50,8 +50,6 @@ struct Cache {
 // map                                                                //
 // ------------------------------------------------------------------ //
 
-constexpr int MAP_THREADS = 256;
-
 struct MapArgs {
     const int *len, *start, *end;
     int n;
@@ -94,66 +92,83 @@ __host__ __device__ __forceinline__ int pages_of(const Div &page, int x)
 // it, the old table entry; a new block's page that a row needs is looked up
 // like the pop that writes it. *n_free is replaced by the last CTA to have
 // read it.
-__global__ void __launch_bounds__(MAP_THREADS) map_kernel(const MapArgs a)
+//
+// A step of few rows is one CTA and bound by its chain of three loads from
+// memory (lengths, pages, then the rows' stores); many rows are bound by
+// their 12 bytes each: a thread then finds the request of ROWS = 4 rows with
+// one search and stores them in 16 bytes.
+template <int THREADS, int ROWS>
+__global__ void __launch_bounds__(THREADS) map_kernel(const MapArgs a)
 {
-    extern __shared__ int sums[];  // [3][n + 1]
-    __shared__ long long wsum[3][MAP_THREADS / 32];
-    __shared__ int any_bad, had_s;
+    constexpr int W = THREADS / 32;
+    extern __shared__ int sums[];  // [3][n + 1], then [3][n]
+    __shared__ uint4 warp_sum[W], warp_much[W];
+    __shared__ int had_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.n;
     int *rows = sums, *push = sums + (n + 1), *pop = sums + 2 * (n + 1);
-    if (tid == 0) {
-        any_bad = 0;
-        had_s = *a.n_free;
-    }
-    __syncthreads();
+    int *starts = sums + 3 * (n + 1), *helds = starts + n, *ends = helds + n;  // helds: pages of len
+    if (tid == 0) had_s = *a.n_free;
     const long long most = (long long)a.c.max_blocks * a.c.page.d;
-    const int per = (n + MAP_THREADS - 1) / MAP_THREADS, i0 = min(n, tid * per), i1 = min(n, i0 + per);
-    long long s[3] = {0, 0, 0};
     bool bad = false;
-    for (int i = i0; i < i1; i++) {
+    for (int i = tid; i < n; i += THREADS) {
         const int len = a.len[i], st = a.start[i], en = a.end[i];
-        if (st < 0 || st > len || en < st || en > most || len > most) {
-            bad = true;
-            continue;
-        }
-        const int d = pages_of(a.c.page, en) - pages_of(a.c.page, len);
-        s[0] += en - st;
-        s[1] += max(0, -d);
-        s[2] += max(0, d);
+        bad |= st < 0 || st > len || en < st || en > most || len > most;
+        starts[i] = st;
+        helds[i] = pages_of(a.c.page, len);
+        ends[i] = en;
     }
-    if (bad) any_bad = 1;
-    long long e[3];
+    const bool any_bad = __syncthreads_or(bad);
+    const int per = (n + THREADS - 1) / THREADS, i0 = min(n, tid * per), i1 = any_bad ? i0 : min(n, i0 + per);
+    // sums in 32 bits, and beside them those of 4096ths, which cannot
+    // overflow (4096 requests of at most 2^30)
+    unsigned own[3] = {0, 0, 0}, much[3] = {0, 0, 0};
+    for (int i = i0; i < i1; i++) {
+        const int d = pages_of(a.c.page, ends[i]) - helds[i];
+        const unsigned x[3] = {(unsigned)(ends[i] - starts[i]), (unsigned)max(0, -d), (unsigned)max(0, d)};
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            own[k] += x[k];
+            much[k] += x[k] >> 12;
+        }
+    }
+    unsigned e[3], tot[3], big[3];
 #pragma unroll
     for (int k = 0; k < 3; k++) {
-        long long v = s[k];
+        e[k] = own[k];
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xFFFFFFFFu, v, o);
-            if (lane >= o) v += u;
+            const unsigned u = __shfl_up_sync(0xFFFFFFFFu, e[k], o);
+            if (lane >= o) e[k] += u;
         }
-        if (lane == 31) wsum[k][warp] = v;
-        e[k] = v - s[k];
+        much[k] = __reduce_add_sync(0xFFFFFFFFu, much[k]);
+    }
+    if (lane == 31) {
+        warp_sum[warp] = make_uint4(e[0], e[1], e[2], 0u);
+        warp_much[warp] = make_uint4(much[0], much[1], much[2], 0u);
     }
     __syncthreads();
-    long long tot[3];
+    {
+        const uint4 x = lane < W ? warp_sum[lane] : make_uint4(0, 0, 0, 0), y = lane < W ? warp_much[lane] : make_uint4(0, 0, 0, 0);
+        const unsigned xs[3] = {x.x, x.y, x.z}, ys[3] = {y.x, y.y, y.z};
 #pragma unroll
-    for (int k = 0; k < 3; k++) {
-        long long t = 0;
-        for (int w = 0; w < MAP_THREADS / 32; w++) {
-            if (w == warp) e[k] += t;
-            t += wsum[k][w];
+        for (int k = 0; k < 3; k++) {
+            e[k] += __reduce_add_sync(0xFFFFFFFFu, lane < warp ? xs[k] : 0u) - own[k];
+            tot[k] = __reduce_add_sync(0xFFFFFFFFu, xs[k]);
+            big[k] = __reduce_add_sync(0xFFFFFFFFu, ys[k]);
         }
-        tot[k] = t;
     }
+    // a sum over 2^30, as all limits are, is one that cannot be met
+    const unsigned over = (1u << 18) + 4096u;  // (big + requests) 4096ths hold the sum
+    const bool far0 = big[0] >= over, far1 = big[1] >= over, far2 = big[2] >= over;
     const int had = had_s;
     int code = 0;
-    if (any_bad || had < 0 || had > a.c.n_pages) {
+    if (any_bad || had < 0 || had > a.c.n_pages || far1) {
         code = KV_PAGED_BAD_LENGTH;
     } else {
-        if (tot[0] > a.max_rows) code |= KV_PAGED_NO_ROWS;
-        if (tot[2] > had + tot[1]) {
+        if (far0 || tot[0] > (unsigned)a.max_rows) code |= KV_PAGED_NO_ROWS;
+        if (far2 || tot[2] > had + tot[1]) {
             code |= KV_PAGED_NO_PAGES;
-        } else if (had + tot[1] - tot[2] > a.c.n_pages) {
+        } else if (had + tot[1] - tot[2] > (unsigned)a.c.n_pages) {
             code |= KV_PAGED_BAD_LENGTH;  // more pages given back than the pool has
         }
     }
@@ -161,12 +176,11 @@ __global__ void __launch_bounds__(MAP_THREADS) map_kernel(const MapArgs a)
     const int top = had + n_push;  // the stack's height between the pushes and the pops
     if (!code) {
         for (int i = i0; i < i1; i++) {
-            const int st = a.start[i], en = a.end[i];
-            const int d = pages_of(a.c.page, en) - pages_of(a.c.page, a.len[i]);
+            const int d = pages_of(a.c.page, ends[i]) - helds[i];
             rows[i] = (int)e[0];
             push[i] = (int)e[1];
             pop[i] = (int)e[2];
-            e[0] += en - st;
+            e[0] += ends[i] - starts[i];
             e[1] += max(0, -d);
             e[2] += max(0, d);
         }
@@ -180,44 +194,67 @@ __global__ void __launch_bounds__(MAP_THREADS) map_kernel(const MapArgs a)
     // the page of push `x`, where its request still holds it
     auto pushed = [&](int x) {
         const int i = find_request(push, n, x);
-        return a.table[(size_t)i * a.c.max_blocks + pages_of(a.c.page, a.end[i]) + (x - push[i])];
+        return a.table[(size_t)i * a.c.max_blocks + pages_of(a.c.page, ends[i]) + (x - push[i])];
     };
     // the page that pop `x` takes
     auto popped = [&](int x) {
         const int p = top - 1 - x;
         return p >= had ? pushed(p - had) : a.free_pages[p];
     };
-    const int gid = blockIdx.x * MAP_THREADS + tid, gsz = gridDim.x * MAP_THREADS;
+    const int gid = blockIdx.x * THREADS + tid, gsz = gridDim.x * THREADS;
     int found = code;
-    if (blockIdx.x == 0) {
-        for (int i = tid; i <= n; i += MAP_THREADS) a.row0[i] = code ? 0 : rows[i];
+    // rows first: they read what the pushes and pops below, of any CTA, leave alone
+    const bool wide = ((((uintptr_t)a.row_request | (uintptr_t)a.row_pos | (uintptr_t)a.row_slot) & 15) == 0);
+    for (int r0 = ROWS * gid; r0 < a.max_rows; r0 += ROWS * gsz) {
+        int req[ROWS], pos[ROWS], slot[ROWS];
+        int q = r0 < n_rows ? find_request(rows, n, r0) : n, blk = -1, page = -1;
+#pragma unroll
+        for (int k = 0; k < ROWS; k++) {
+            const int r = r0 + k;
+            req[k] = pos[k] = slot[k] = -1;
+            if (r >= n_rows) continue;
+            while (r >= rows[q + 1]) {
+                q++;
+                blk = -1;
+            }
+            const int p = starts[q] + (r - rows[q]);
+            if (blk < 0 || p - blk * (int)a.c.page.d >= (int)a.c.page.d) {
+                blk = div_by(a.c.page, p);
+                page = blk < helds[q] ? a.table[(size_t)q * a.c.max_blocks + blk] : popped(pop[q] + blk - helds[q]);
+                if (page < 0 || page >= a.c.n_pages) found |= KV_PAGED_BAD_PAGE;
+            }
+            req[k] = q;
+            pos[k] = p;
+            if (page >= 0 && page < a.c.n_pages) slot[k] = page * (int)a.c.page.d + (p - blk * (int)a.c.page.d);
+        }
+        if (ROWS == 4 && wide && r0 + ROWS <= a.max_rows) {
+            *reinterpret_cast<int4 *>(a.row_request + r0) = make_int4(req[0], req[1 % ROWS], req[2 % ROWS], req[3 % ROWS]);
+            *reinterpret_cast<int4 *>(a.row_pos + r0) = make_int4(pos[0], pos[1 % ROWS], pos[2 % ROWS], pos[3 % ROWS]);
+            *reinterpret_cast<int4 *>(a.row_slot + r0) = make_int4(slot[0], slot[1 % ROWS], slot[2 % ROWS], slot[3 % ROWS]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < ROWS; k++) {
+                if (r0 + k >= a.max_rows) break;
+                a.row_request[r0 + k] = req[k];
+                a.row_pos[r0 + k] = pos[k];
+                a.row_slot[r0 + k] = slot[k];
+            }
+        }
     }
-    for (int x = gid; x < top - n_pop - had; x += gsz) {
+    if (blockIdx.x == 0) {
+        for (int i = tid; i <= n; i += THREADS) a.row0[i] = code ? 0 : rows[i];
+    }
+    // the pushes and pops begin at the last threads, which have no rows in most steps
+    const int back = gsz - 1 - gid;
+    for (int x = back; x < top - n_pop - had; x += gsz) {
         const int p = pushed(x);
         if (p < 0 || p >= a.c.n_pages) found |= KV_PAGED_BAD_PAGE;
         a.free_pages[had + x] = p;
     }
-    for (int x = gid; x < n_pop; x += gsz) {
+    for (int x = back; x < n_pop; x += gsz) {
         const int i = find_request(pop, n, x), p = popped(x);
         if (p < 0 || p >= a.c.n_pages) found |= KV_PAGED_BAD_PAGE;
-        a.table[(size_t)i * a.c.max_blocks + pages_of(a.c.page, a.len[i]) + (x - pop[i])] = p;
-    }
-    for (int r = gid; r < a.max_rows; r += gsz) {
-        int req = -1, pos = -1, slot = -1;
-        if (r < n_rows) {
-            req = find_request(rows, n, r);
-            pos = a.start[req] + (r - rows[req]);
-            const int blk = div_by(a.c.page, pos), held = pages_of(a.c.page, a.len[req]);
-            const int p = blk < held ? a.table[(size_t)req * a.c.max_blocks + blk] : popped(pop[req] + blk - held);
-            if (p < 0 || p >= a.c.n_pages) {
-                found |= KV_PAGED_BAD_PAGE;
-            } else {
-                slot = p * (int)a.c.page.d + (pos - blk * (int)a.c.page.d);
-            }
-        }
-        a.row_request[r] = req;
-        a.row_pos[r] = pos;
-        a.row_slot[r] = slot;
+        a.table[(size_t)i * a.c.max_blocks + helds[i] + (x - pop[i])] = p;
     }
     if (found) atomicOr(a.err, found);
     if (tid == 0) {
@@ -242,51 +279,79 @@ struct AppendArgs {
     const float *rope_cs;
     int rope_dim, rope_len, heads, kv_heads, hs;
     uint64_t q_stride, kv_stride, q_out_stride;
+    Div hs4;  // head size / 4
     Cache c;
     int *err;
 };
 
-template <typename KV>
-__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a)
+constexpr int APP_THREADS = 256, APP_AHEAD = 4;
+
+// Four entries, rounded as the cache holds them.
+__device__ __forceinline__ void kv_store4(float *p, float4 v)
 {
-    const int r = blockIdx.x, slot = a.row_slot[r], pos = a.row_pos[r];
-    if (slot < 0) return;
-    if (slot >= a.c.n_pages * (int)a.c.page.d || (a.rope_dim > 0 && (pos < 0 || pos >= a.rope_len))) {
-        if (threadIdx.x == 0) atomicOr(a.err, KV_PAGED_BAD_ROW);
-        return;
-    }
-    const int page = div_by(a.c.page, slot), place = slot - page * (int)a.c.page.d;
-    const float *rope = a.rope_cs + (size_t)pos * a.rope_dim;
-    KV *kp = static_cast<KV *>(a.k_pool) + page * a.c.page_stride + place * a.c.token_stride;
-    KV *vp = static_cast<KV *>(a.v_pool) + page * a.c.page_stride + place * a.c.token_stride;
-    auto turn = [&](const float *x, int d, float &x0, float &x1) {
-        x0 = x[0];
-        x1 = x[1];
-        if (d < a.rope_dim) {
-            const float c = rope[d], sn = rope[d + 1];
-            const float t = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, sn));
-            x1 = __fadd_rn(__fmul_rn(x0, sn), __fmul_rn(x1, c));
-            x0 = t;
+    *reinterpret_cast<float4 *>(p) = v;
+}
+__device__ __forceinline__ void kv_store4(__half *p, float4 v)
+{
+    const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+    *reinterpret_cast<uint2 *>(p) =
+        make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+}
+
+// CTA (r, y) takes every gridDim.y-th stretch of row r's q, k and v, in 16
+// bytes a thread, APP_AHEAD loads in flight: a copy, bound by memory. A
+// pair's two products and their sum are each rounded, as the decode step
+// does.
+template <typename KV>
+__global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
+{
+    const int r = blockIdx.x;
+    const int q4 = a.q != nullptr ? a.heads * a.hs / 4 : 0, k4 = a.kv_heads * a.hs / 4, all = q4 + 2 * k4;
+    const int step = gridDim.y * APP_THREADS;
+    const float *q = a.q + r * a.q_stride, *k = a.k + r * a.kv_stride, *v = a.v + r * a.kv_stride;
+    const int slot = a.row_slot[r], pos = a.row_pos[r];  // used once the first loads are under way
+    int page = 0, place = 0;
+    for (int i0 = blockIdx.y * APP_THREADS + threadIdx.x; i0 < all; i0 += APP_AHEAD * step) {
+        float4 x[APP_AHEAD];
+#pragma unroll
+        for (int j = 0; j < APP_AHEAD; j++) {
+            const int i = i0 + j * step;
+            if (i < all) x[j] = __ldcs(reinterpret_cast<const float4 *>(i < q4 ? q + 4 * i : i < q4 + k4 ? k + 4 * (i - q4) : v + 4 * (i - q4 - k4)));
         }
-    };
-    if (a.q != nullptr) {
-        for (int p = threadIdx.x; p < a.heads * a.hs / 2; p += blockDim.x) {
-            float x0, x1;
-            turn(a.q + r * a.q_stride + 2 * p, 2 * p % a.hs, x0, x1);
-            float *o = a.q_out + r * a.q_out_stride + 2 * p;
-            o[0] = x0;
-            o[1] = x1;
+        if (i0 < APP_AHEAD * step) {
+            if (slot < 0) return;
+            if (slot >= a.c.n_pages * (int)a.c.page.d || (a.rope_dim > 0 && (pos < 0 || pos >= a.rope_len))) {
+                if (threadIdx.x == 0) atomicOr(a.err, KV_PAGED_BAD_ROW);
+                return;
+            }
+            page = div_by(a.c.page, slot);
+            place = slot - page * (int)a.c.page.d;
         }
-    }
-    for (int p = threadIdx.x; p < a.kv_heads * a.hs / 2; p += blockDim.x) {
-        const int h = 2 * p / a.hs, d = 2 * p - h * a.hs;
-        float x0, x1;
-        turn(a.k + r * a.kv_stride + 2 * p, d, x0, x1);
-        kv_store(kp, h * a.c.head_stride + d, x0);
-        kv_store(kp, h * a.c.head_stride + d + 1, x1);
-        const float *v = a.v + r * a.kv_stride + 2 * p;
-        kv_store(vp, h * a.c.head_stride + d, v[0]);
-        kv_store(vp, h * a.c.head_stride + d + 1, v[1]);
+        const float *rope = a.rope_cs + (size_t)pos * a.rope_dim;
+        const uint64_t at = page * a.c.page_stride + place * a.c.token_stride;
+#pragma unroll
+        for (int j = 0; j < APP_AHEAD; j++) {
+            const int i = i0 + j * step;
+            if (i >= all) break;
+            const int part = i < q4 ? 0 : i < q4 + k4 ? 1 : 2, e = i - (part == 0 ? 0 : part == 1 ? q4 : q4 + k4);
+            const int h = div_by(a.hs4, e), d = 4 * (e - h * (int)a.hs4.d);
+            float4 y = x[j];
+            if (part < 2 && d < a.rope_dim) {
+                const float2 cs = __ldg(reinterpret_cast<const float2 *>(rope + d));
+                y.x = __fsub_rn(__fmul_rn(x[j].x, cs.x), __fmul_rn(x[j].y, cs.y));
+                y.y = __fadd_rn(__fmul_rn(x[j].x, cs.y), __fmul_rn(x[j].y, cs.x));
+                if (d + 2 < a.rope_dim) {
+                    const float2 ds = __ldg(reinterpret_cast<const float2 *>(rope + d + 2));
+                    y.z = __fsub_rn(__fmul_rn(x[j].z, ds.x), __fmul_rn(x[j].w, ds.y));
+                    y.w = __fadd_rn(__fmul_rn(x[j].z, ds.y), __fmul_rn(x[j].w, ds.x));
+                }
+            }
+            if (part == 0) {
+                *reinterpret_cast<float4 *>(a.q_out + r * a.q_out_stride + 4 * e) = y;
+            } else {
+                kv_store4(static_cast<KV *>(part == 1 ? a.k_pool : a.v_pool) + at + h * a.c.head_stride + d, y);
+            }
+        }
     }
 }
 
@@ -1091,8 +1156,8 @@ static const char *shape_fault(KvPagedShape &s)
     if (s.n_heads < 1 || s.n_kv_heads < 1 || s.n_heads % s.n_kv_heads || s.n_heads > 65535)
         return "The query heads must be a multiple of the key-value heads, at most 65535.";
     if (s.head_size < 8 || s.head_size > 256 || s.head_size % 8) return "The head size must be a multiple of 8, 8 to 256.";
-    if (s.page_tokens < 1 || s.n_pages < 1 || (long long)s.page_tokens * s.n_pages > 0x7FFFFFFFll)
-        return "Pages and page size must be positive, with less than 2^31 tokens in all.";
+    if (s.page_tokens < 1 || s.n_pages < 1 || (long long)s.page_tokens * s.n_pages > 1ll << 30)
+        return "Pages and page size must be positive, with at most 2^30 tokens in all.";
     if (s.max_requests < 1 || s.max_requests > KV_PAGED_MAX_REQUESTS)
         return "The block table takes 1 to 4096 requests.";
     if (s.max_blocks < 1 || (long long)s.max_blocks * s.page_tokens > 1ll << 30)
@@ -1221,9 +1286,12 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
         const size_t flags = 256 + (((size_t)kv->grid * 4 + 255) & ~(size_t)255);
         if (e == cudaSuccess) e = cudaMalloc(&kv->scratch, flags + parts);
         if (e == cudaSuccess) e = cudaMemset(kv->scratch, 0, flags);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(kvp::map_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     3 * (KV_PAGED_MAX_REQUESTS + 1) * 4);
+        const int map_smem = (6 * s.max_requests + 3) * 4;
+        if (e == cudaSuccess && map_smem > 48 * 1024) {
+            e = cudaFuncSetAttribute(kvp::map_kernel<1024, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, map_smem);
+            if (e == cudaSuccess)
+                e = cudaFuncSetAttribute(kvp::map_kernel<1024, 4>, cudaFuncAttributeMaxDynamicSharedMemorySize, map_smem);
+        }
         kv->err = (int *)kv->scratch;
         kv->map_arrived = (unsigned *)kv->scratch + 32;
         kv->arrived = (unsigned *)(kv->scratch + 256);
@@ -1276,18 +1344,27 @@ extern "C" int kv_paged_map(KvPaged *kv, const int *len, const int *start, const
     if (!len || !start || !end || !table || !free_pages || !n_free || !n_free_out || !row0)
         return refuse(kv, "map: a pointer is NULL.");
     if (n < 1 || n > kv->s.max_requests) return refuse(kv, "map: requests outside 1 .. max_requests.");
-    if (max_rows < 0 || (max_rows > 0 && (!row_request || !row_pos || !row_slot)))
+    if (max_rows < 0 || max_rows > 1 << 30 || (max_rows > 0 && (!row_request || !row_pos || !row_slot)))
         return refuse(kv, "map: no room for the rows.");
     if (kv->device < 0) return refuse(kv, "The handle has no device.");
     OnDevice on(kv->device);
     if (!on.ok) return refuse(kv, "CUDA device cannot be used.");
     kvp::MapArgs a = {len, start, end, n, table, free_pages, n_free, n_free_out, max_rows, row_request, row_pos,
                       row_slot, row0, kv->c, kv->map_arrived, kv->err};
-    int grid = (max_rows + 4 * kvp::MAP_THREADS - 1) / (4 * kvp::MAP_THREADS);
-    if (grid > 2 * kv->sms) grid = 2 * kv->sms;
-    if (grid < 1) grid = 1;
+    // Every CTA sums over all requests, so many of those take wide CTAs; four
+    // rows a thread when one each would be more than the threads resident at once.
     cudaGetLastError();
-    kvp::map_kernel<<<grid, kvp::MAP_THREADS, 3 * (n + 1) * 4, (cudaStream_t)stream>>>(a);
+    auto go = [&](auto kernel, int threads, int rows) {
+        const int most = kv->sms * (threads == 1024 ? 2 : 4);
+        const long long ctas = ((long long)max_rows + (long long)rows * threads - 1) / ((long long)rows * threads);
+        kernel<<<(int)(ctas < 1 ? 1 : ctas < most ? ctas : most), threads, (6 * n + 3) * 4, (cudaStream_t)stream>>>(a);
+    };
+    const bool many = max_rows > kv->sms * 1024;
+    if (n > 1024) {
+        many ? go(kvp::map_kernel<1024, 4>, 1024, 4) : go(kvp::map_kernel<1024, 1>, 1024, 1);
+    } else {
+        many ? go(kvp::map_kernel<256, 4>, 256, 4) : go(kvp::map_kernel<256, 1>, 256, 1);
+    }
     return launched(kv, "map");
 }
 
@@ -1316,12 +1393,18 @@ extern "C" int kv_paged_append(KvPaged *kv, const float *q, const float *k, cons
     OnDevice on(kv->device);
     if (!on.ok) return refuse(kv, "CUDA device cannot be used.");
     kvp::AppendArgs a = {q, k, v, row_pos, row_slot, q_out, k_pool, v_pool, rope_cs, rope_dim, rope_len, s.n_heads,
-                         s.n_kv_heads, s.head_size, q_stride, kv_stride, q_out == q ? q_stride : qd, kv->c, kv->err};
+                         s.n_kv_heads, s.head_size, q_stride, kv_stride, q_out == q ? q_stride : qd, kvp::make_div((uint32_t)s.head_size / 4),
+                         kv->c, kv->err};
+    // few rows are split, up to a pass of all threads over a row, until they fill the SMs twice
+    const int passes = (int)(((q ? qd : 0) + 2 * kvd + 4 * kvp::APP_THREADS - 1) / (4 * kvp::APP_THREADS));
+    int split = (2 * kv->sms + n - 1) / n;
+    if (split > passes) split = passes;
+    const dim3 grid(n, split);
     cudaGetLastError();
     if (s.type == 1) {
-        kvp::append_kernel<__half><<<n, 256, 0, (cudaStream_t)stream>>>(a);
+        kvp::append_kernel<__half><<<grid, kvp::APP_THREADS, 0, (cudaStream_t)stream>>>(a);
     } else {
-        kvp::append_kernel<float><<<n, 256, 0, (cudaStream_t)stream>>>(a);
+        kvp::append_kernel<float><<<grid, kvp::APP_THREADS, 0, (cudaStream_t)stream>>>(a);
     }
     return launched(kv, "append");
 }
