@@ -119,6 +119,30 @@ int engine_launches_per_step(const LLMModel *model);
  * error. */
 int engine_batch_open(LLMModel *model, int max_seqs, char *error, size_t error_capacity);
 
+/* engine_batch_open with the sequences' caches in pages: one pool of n_pages
+ * pages of page_tokens positions (both >= 1) serves all max_seqs sequences,
+ * each of which may grow to the model's context while pages are left
+ * (n_pages * page_tokens * the model's bytes per position, instead of
+ * max_seqs whole contexts). engine_forward_batch and engine_kv_write work as
+ * on engine_batch_open's state, with three differences. The rows of one sequence in a
+ * call are consecutive positions. The sequence ends with the last of them:
+ * a row at a position that was filled before takes back the positions behind
+ * it (a rejected draft, or position 0 for a new text), and their pages. A
+ * call that needs more pages than are free returns 0 with a message and
+ * changes nothing. Head sizes that are multiples of 8; one GPU. Block
+ * tables, appends and attention run on the device (kv_paged.h). Returns 1,
+ * or 0 with a message in error. */
+int engine_batch_open_paged(LLMModel *model, int max_seqs, int page_tokens, int n_pages, char *error,
+                            size_t error_capacity);
+
+/* Sequence `seq` of the batched state starts over at position 0; on a paged
+ * state its pages are free for others. Returns 1, or 0 for a sequence that is not
+ * there or a device error (engine_last_error). */
+int engine_batch_release(LLMModel *model, int seq);
+
+/* Pages of a paged state that no sequence holds, -1 without such a state. */
+int engine_batch_free_pages(const LLMModel *model);
+
 /* One step over n <= 64 rows: sequence seq_ids[i] consumes tokens[i] at
  * position pos[i] (seq_ids below max_seqs; tokens in the vocabulary;
  * positions below the context length; each (sequence, position) at most

@@ -108,6 +108,7 @@ struct LLMModel {
     int tp_world;      /* tensor-parallel ranks (1: single GPU) */
     int connected;     /* the decode step exists (tensor parallel: after engine_tp_connect) */
     int batch_seqs;    /* sequences of the batched state */
+    int batch_paged;   /* the batched state's caches are pages of one pool */
     int kv_half;       /* KV cache entries in IEEE half (POCKET_CUDA_KV=f16) */
     int kv_head0, kv_heads;  /* this rank's KV heads (all of them on one GPU) */
     int *filled;       /* batched sequences: positions 0 .. filled[s] - 1 hold K/V */
@@ -965,7 +966,7 @@ int engine_generate_greedy(LLMModel *m, int token, int pos, int n, int *out_toke
     return 1;
 }
 
-int engine_batch_open(LLMModel *m, int max_seqs, char *err, size_t cap)
+static int batch_open(LLMModel *m, int max_seqs, int paged, int page_tokens, int n_pages, char *err, size_t cap)
 {
     if (m == NULL || m->dev == NULL || !m->connected) {
         seterr(err, cap, "No model.");
@@ -983,11 +984,39 @@ int engine_batch_open(LLMModel *m, int max_seqs, char *err, size_t cap)
         seterr(err, cap, "Out of memory.");
         return 0;
     }
-    m->batch = pkb_create(m->dev, max_seqs, err, cap);
+    m->batch = paged ? pkb_create_paged(m->dev, max_seqs, page_tokens, n_pages, err, cap)
+                     : pkb_create(m->dev, max_seqs, err, cap);
     if (m->batch == NULL) return 0;
     m->batch_seqs = max_seqs;
+    m->batch_paged = paged;
     if (err && cap) err[0] = '\0';
     return 1;
+}
+
+int engine_batch_open(LLMModel *m, int max_seqs, char *err, size_t cap)
+{
+    return batch_open(m, max_seqs, 0, 0, 0, err, cap);
+}
+
+int engine_batch_open_paged(LLMModel *m, int max_seqs, int page_tokens, int n_pages, char *err, size_t cap)
+{
+    return batch_open(m, max_seqs, 1, page_tokens, n_pages, err, cap);
+}
+
+int engine_batch_release(LLMModel *m, int seq)
+{
+    if (m == NULL || m->batch == NULL || seq < 0 || seq >= m->batch_seqs) return 0;
+    if (m->batch_paged && !pkb_release(m->batch, seq)) {
+        snprintf(m->last_error, sizeof(m->last_error), "%s", pkb_error(m->batch));
+        return 0;
+    }
+    m->filled[seq] = 0;
+    return 1;
+}
+
+int engine_batch_free_pages(const LLMModel *m)
+{
+    return m == NULL || m->batch == NULL ? -1 : pkb_free_pages(m->batch);
 }
 
 int engine_forward_batch(LLMModel *m, const int *tokens, const int *pos, const int *seq_ids, int n,
@@ -1019,10 +1048,27 @@ int engine_forward_batch(LLMModel *m, const int *tokens, const int *pos, const i
             return 0;
         }
     }
+    /* A paged sequence ends with the last of its rows, so these are
+     * consecutive positions. */
+    for (int i = 0; m->batch_paged && i < n; i++) {
+        int lo = pos[i], hi = pos[i], rows = 0;
+        for (int j = 0; j < n; j++) {
+            if (seq_ids[j] != seq_ids[i]) continue;
+            rows++;
+            if (pos[j] < lo) lo = pos[j];
+            if (pos[j] > hi) hi = pos[j];
+        }
+        if (hi - lo + 1 != rows) {
+            snprintf(m->last_error, sizeof(m->last_error),
+                     "Sequence %d's rows are not consecutive positions (%d rows in %d .. %d).", seq_ids[i], rows, lo, hi);
+            return 0;
+        }
+    }
     if (!pkb_step(m->batch, tokens, pos, seq_ids, n, next_tokens, logits)) {
         snprintf(m->last_error, sizeof(m->last_error), "%s", pkb_error(m->batch));
         return 0;
     }
+    for (int i = 0; m->batch_paged && i < n; i++) m->filled[seq_ids[i]] = 0;
     for (int i = 0; i < n; i++)
         if (pos[i] + 1 > m->filled[seq_ids[i]]) m->filled[seq_ids[i]] = pos[i] + 1;
     return 1;

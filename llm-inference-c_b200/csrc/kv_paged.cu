@@ -10,6 +10,7 @@
 #include <string.h>
 
 #include "kv_paged.h"
+#include "kv_paged_dev.h"
 #include "pk_quant.cuh"
 
 namespace pk {
@@ -1320,6 +1321,11 @@ extern "C" void kv_paged_close(KvPaged *kv)
 extern "C" const char *kv_paged_last_error(const KvPaged *kv)
 {
     return kv ? kv->msg : "";
+}
+
+const int *kv_paged_error_word(const KvPaged *kv)
+{
+    return kv->err;
 }
 
 extern "C" int kv_paged_error(KvPaged *kv)

@@ -18,7 +18,9 @@
 // graph (inputs and outputs through fixed pinned buffers).
 //
 // KV caches: [sequence][layer][position][kv_dim] fp32, as the reference's
-// run state (src/transformer.c: key_cache / value_cache) per sequence.
+// run state (src/transformer.c: key_cache / value_cache) per sequence. A
+// paged state (pkb_create_paged) keeps a pool of pages per layer instead,
+// and steps through kv_paged.h.
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -26,6 +28,8 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include "kv_paged.h"
+#include "kv_paged_dev.h"
 #include "pk_dev.h"
 #include "pk_mma.h"
 #include "pk_quant.cuh"
@@ -799,6 +803,15 @@ struct PkbCtx {
     int kv_alias;  // kc / vc belong to the decode step (pkb_create_prefill): not freed here
     cudaStream_t side;             // tile-kernel matrices that run beside a tensor-core launch
     cudaEvent_t ev_fork, ev_join;  //   (forked from and joined to st inside the captured step)
+    // paged state (paged != NULL): kc / vc are [L][n_pages][page_tokens][kvd]
+    KvPaged *paged;
+    int page_tokens, n_pages, blocks;  // blocks: pages of a whole context
+    int len[bt::BMAX];                 // tokens of each sequence that hold pages
+    int *pg_h, *pg_d;                  // a step's [len 64][start 64][end 64]
+    int *table, *free_pages, *n_free;  // [max_seqs][blocks], [n_pages], [1]
+    int *rows;                         // map's rows: [request][position][slot] of row_cap each, then row0
+    int row_cap;
+    float *kv_stage;                   // pkb_kv_write's rows on the device: [2][KV_STAGE][kvd]
     char msg[256];
 };
 
@@ -806,6 +819,95 @@ static int bfail(PkbCtx *b, cudaError_t e, const char *what)
 {
     if (e == cudaSuccess) return 0;
     snprintf(b->msg, sizeof(b->msg), "CUDA %s failed: %s", what, cudaGetErrorString(e));
+    return 1;
+}
+
+constexpr int KV_STAGE = 256;  // rows that pkb_kv_write carries to the device at a time
+
+static int pages_for(const PkbCtx *b, int tokens)
+{
+    return (tokens + b->page_tokens - 1) / b->page_tokens;
+}
+
+// Pages of a paged state that no sequence holds.
+static int pages_left(const PkbCtx *b)
+{
+    int used = 0;
+    for (int s = 0; s < b->max_seqs; s++) used += pages_for(b, b->len[s]);
+    return b->n_pages - used;
+}
+
+// kv_paged_map on the state's stream, for the lengths in pg_d.
+static int paged_map(PkbCtx *b, int max_rows)
+{
+    const int B = bt::BMAX, C = b->row_cap;
+    if (kv_paged_map(b->paged, b->pg_d, b->pg_d + B, b->pg_d + 2 * B, b->max_seqs, b->table, b->free_pages, b->n_free,
+                     b->n_free, max_rows, b->rows, b->rows + C, b->rows + 2 * C, b->rows + 3 * C, b->st))
+        return 1;
+    snprintf(b->msg, sizeof(b->msg), "%s", kv_paged_last_error(b->paged));
+    return 0;
+}
+
+// Gives sequence `seq` the pages of tokens [0, end), with its rows from
+// `start` on in `rows`; the others stay as they are. Waits for it.
+static int paged_resize(PkbCtx *b, int seq, int start, int end, int max_rows)
+{
+    const int B = bt::BMAX, len = b->len[seq];
+    if (pages_for(b, end) - pages_for(b, len) > pages_left(b)) {
+        snprintf(b->msg, sizeof(b->msg), "Not enough free pages: %d needed, %d left.",
+                 pages_for(b, end) - pages_for(b, len), pages_left(b));
+        return 0;
+    }
+    for (int s = 0; s < b->max_seqs; s++) {
+        b->pg_h[s] = b->len[s];
+        b->pg_h[B + s] = s == seq ? start : b->len[s];
+        b->pg_h[2 * B + s] = s == seq ? end : b->len[s];
+    }
+    if (bfail(b, cudaMemcpyAsync(b->pg_d, b->pg_h, (size_t)(3 * B) * 4, cudaMemcpyHostToDevice, b->st), "page copy") ||
+        !paged_map(b, max_rows) || bfail(b, cudaStreamSynchronize(b->st), "page map"))
+        return 0;
+    const int bits = kv_paged_error(b->paged);
+    if (bits != 0) {
+        snprintf(b->msg, sizeof(b->msg), "The page map was refused (error word %d).", bits);
+        return 0;
+    }
+    b->len[seq] = end;
+    return 1;
+}
+
+extern "C" int pkb_release(PkbCtx *b, int seq)
+{
+    cudaSetDevice(b->device);
+    return paged_resize(b, seq, 0, 0, 0);
+}
+
+extern "C" int pkb_free_pages(const PkbCtx *b)
+{
+    return b->paged ? pages_left(b) : -1;
+}
+
+// pkb_kv_write of a paged state: the rows' pages, then their entries,
+// KV_STAGE rows at a time.
+static int paged_kv_write(PkbCtx *b, int seq, int layer, int pos0, int npos, const float *k, const float *v)
+{
+    const PkdModel &m = b->m;
+    const size_t kvd = (size_t)m.head_size * (size_t)m.n_kv_heads;
+    const int end = pos0 + npos > b->len[seq] ? pos0 + npos : b->len[seq], C = b->row_cap;
+    if (!paged_resize(b, seq, pos0, end, end - pos0)) return 0;
+    const size_t pool = (size_t)b->n_pages * b->page_tokens * kvd * (m.kv_half ? 2 : 4) * (size_t)layer;
+    for (int i = 0; i < npos; i += KV_STAGE) {
+        const int n = npos - i < KV_STAGE ? npos - i : KV_STAGE;
+        float *dk = b->kv_stage, *dv = b->kv_stage + KV_STAGE * kvd;
+        if (bfail(b, cudaMemcpyAsync(dk, k + i * kvd, n * kvd * 4, cudaMemcpyHostToDevice, b->st), "KV write") ||
+            bfail(b, cudaMemcpyAsync(dv, v + i * kvd, n * kvd * 4, cudaMemcpyHostToDevice, b->st), "KV write"))
+            return 0;
+        if (!kv_paged_append(b->paged, NULL, dk, dv, b->rows + C + i, b->rows + 2 * C + i, n, NULL,
+                             (uint8_t *)b->kc + pool, (uint8_t *)b->vc + pool, NULL, 0, 0, 0, 0, b->st)) {
+            snprintf(b->msg, sizeof(b->msg), "%s", kv_paged_last_error(b->paged));
+            return 0;
+        }
+        if (bfail(b, cudaStreamSynchronize(b->st), "KV write")) return 0;
+    }
     return 1;
 }
 
@@ -820,6 +922,11 @@ extern "C" int pkb_kv_write(PkbCtx *b, int seq, int layer, int pos0, int npos, c
         return 0;
     }
     cudaSetDevice(b->device);
+    if (b->paged) {
+        if (paged_kv_write(b, seq, layer, pos0, npos, k, v)) return 1;
+        if (err && cap) snprintf(err, cap, "%s", b->msg);
+        return 0;
+    }
     const size_t kvd = (size_t)m.head_size * (size_t)m.n_kv_heads;
     const size_t off = (((size_t)seq * m.n_layers + layer) * (size_t)m.seq_len + (size_t)pos0) * kvd;
     const size_t n = (size_t)npos * kvd;
@@ -946,6 +1053,22 @@ static void attend(PkbCtx *b, int l, int n, size_t att_smem, KV *kc, KV *vc)
     }
 }
 
+// The same over layer l's pages, for the rows that the step's map made.
+static int attend_paged(PkbCtx *b, int l, int n)
+{
+    const PkdModel &m = b->m;
+    const int C = b->row_cap;
+    const size_t at = (size_t)b->n_pages * b->page_tokens * m.n_kv_heads * m.head_size * (m.kv_half ? 2 : 4) * (size_t)l;
+    uint8_t *kc = (uint8_t *)b->kc + at, *vc = (uint8_t *)b->vc + at;
+    if (kv_paged_append(b->paged, b->q, b->k, b->v, b->rows + C, b->rows + 2 * C, n, b->q, kc, vc,
+                        m.rope_dim > 0 ? b->rope_cs : NULL, m.rope_dim, m.seq_len, 0, 0, b->st) &&
+        kv_paged_attend(b->paged, b->q, kc, vc, b->table, b->max_seqs, b->rows, b->rows + C, n, m.att_scale, b->att, 0,
+                        b->st))
+        return 1;
+    snprintf(b->msg, sizeof(b->msg), "%s", kv_paged_last_error(b->paged));
+    return 0;
+}
+
 // The launches of one step for n sequences (inputs already in io_d).
 // This rank's part of an all-reduce (sum) of len floats at y, in place.
 static void tp_allreduce(PkbCtx *b, float *y, int len, int &idx)
@@ -967,13 +1090,16 @@ static int enqueue_step(PkbCtx *b, int n, int with_logits)
                                         b->x);
     const size_t att_smem = (((size_t)m.seq_len + 3) / 4 * 4 + hs + 128 * 4) * 4;
     int tix = 0;  // this step's tensor-parallel exchanges so far
+    if (b->paged && !paged_map(b, n)) return 0;
     for (int l = 0; l < L; l++) {
         if (l == 0)  // later layers: the residual add and this norm at the end of the previous layer
             bt::rmsnorm_kernel<<<n, 1024, 0, st>>>(b->x, nullptr, b->norms, dim, m.rms_eps, b->xn);
         const PkdTensor *qkv[3] = {&m.wq[l], &m.wk[l], &m.wv[l]};
         float *const qkv_y[3] = {b->q, b->k, b->v};
         if (!bmatmul_group(b, qkv, qkv_y, 3, b->xn, n)) return 0;
-        if (m.kv_half) {
+        if (b->paged) {
+            if (!attend_paged(b, l, n)) return 0;
+        } else if (m.kv_half) {
             attend(b, l, n, att_smem, static_cast<__half *>(b->kc), static_cast<__half *>(b->vc));
         } else {
             attend(b, l, n, att_smem, static_cast<float *>(b->kc), static_cast<float *>(b->vc));
@@ -1013,23 +1139,35 @@ static int enqueue_step(PkbCtx *b, int n, int with_logits)
     }
     // the greedy tokens and the matmul error word come back with the step
     cudaMemcpyAsync(b->io_d + 4 * B, b->mm.err, sizeof(int), cudaMemcpyDeviceToDevice, st);
-    cudaMemcpyAsync(b->io_h + 3 * B, b->io_d + 3 * B, (B + 1) * sizeof(int), cudaMemcpyDeviceToHost, st);
+    if (b->paged)
+        cudaMemcpyAsync(b->io_d + 4 * B + 1, kv_paged_error_word(b->paged), sizeof(int), cudaMemcpyDeviceToDevice, st);
+    cudaMemcpyAsync(b->io_h + 3 * B, b->io_d + 3 * B, (B + 2) * sizeof(int), cudaMemcpyDeviceToHost, st);
     return cudaGetLastError() == cudaSuccess;
 }
 
-static PkbCtx *pkb_create_ex(PkdCtx *ctx, int max_seqs, int alias, char *err, size_t cap);
+static PkbCtx *pkb_create_ex(PkdCtx *ctx, int max_seqs, int alias, int page_tokens, int n_pages, char *err, size_t cap);
 
 extern "C" PkbCtx *pkb_create(PkdCtx *ctx, int max_seqs, char *err, size_t cap)
 {
-    return pkb_create_ex(ctx, max_seqs, 0, err, cap);
+    return pkb_create_ex(ctx, max_seqs, 0, 0, 0, err, cap);
 }
 
 extern "C" PkbCtx *pkb_create_prefill(PkdCtx *ctx, char *err, size_t cap)
 {
-    return pkb_create_ex(ctx, 1, 1, err, cap);
+    return pkb_create_ex(ctx, 1, 1, 0, 0, err, cap);
 }
 
-static PkbCtx *pkb_create_ex(PkdCtx *ctx, int max_seqs, int alias, char *err, size_t cap)
+extern "C" PkbCtx *pkb_create_paged(PkdCtx *ctx, int max_seqs, int page_tokens, int n_pages, char *err, size_t cap)
+{
+    if (page_tokens < 1 || n_pages < 1) {
+        if (err && cap) snprintf(err, cap, "Pages and page size must be positive.");
+        return NULL;
+    }
+    return pkb_create_ex(ctx, max_seqs, 0, page_tokens, n_pages, err, cap);
+}
+
+// page_tokens 0: a contiguous cache per sequence; else a pool of n_pages pages.
+static PkbCtx *pkb_create_ex(PkdCtx *ctx, int max_seqs, int alias, int page_tokens, int n_pages, char *err, size_t cap)
 {
     PkdView v;
     if (!pkd_view(ctx, &v)) {
@@ -1043,6 +1181,10 @@ static PkbCtx *pkb_create_ex(PkdCtx *ctx, int max_seqs, int alias, char *err, si
     const PkdModel &m = *v.model;
     if ((m.head_size & 3) || m.head_size > 256 || m.rope_dim > m.head_size || (m.rope_dim & 1)) {
         if (err && cap) snprintf(err, cap, "Unsupported model shape for batched decode.");
+        return NULL;
+    }
+    if (page_tokens > 0 && v.world > 1) {
+        if (err && cap) snprintf(err, cap, "A paged batch runs on one GPU.");
         return NULL;
     }
     PkbCtx *b = (PkbCtx *)calloc(1, sizeof(PkbCtx));
@@ -1081,7 +1223,22 @@ static PkbCtx *pkb_create_ex(PkdCtx *ctx, int max_seqs, int alias, char *err, si
     cudaSetDevice(b->device);
     cudaDeviceGetAttribute(&b->sms, cudaDevAttrMultiProcessorCount, b->device);
     const int B = bt::BMAX, dim = m.dim, hs = m.head_size, qd = m.n_heads * hs, kvd = m.n_kv_heads * hs;
-    const size_t cache = (size_t)max_seqs * m.n_layers * m.seq_len * kvd * (m.kv_half ? 2 : 4);  // bytes
+    const size_t tokens = page_tokens > 0 ? (size_t)n_pages * page_tokens : (size_t)max_seqs * m.seq_len;
+    const size_t cache = tokens * m.n_layers * kvd * (m.kv_half ? 2 : 4);  // bytes
+    if (page_tokens > 0) {
+        b->page_tokens = page_tokens;
+        b->n_pages = n_pages;
+        b->blocks = (int)(((long long)m.seq_len + page_tokens - 1) / page_tokens);
+        b->row_cap = m.seq_len > B ? m.seq_len : B;
+        const KvPagedShape shape = {m.n_heads, m.n_kv_heads, hs, m.kv_half ? 1u : 0u, page_tokens, n_pages, max_seqs,
+                                    b->blocks, 0, 0, 0};
+        b->paged = kv_paged_open(&shape, b->device, b->msg, sizeof(b->msg));
+        if (b->paged == NULL) {
+            if (err && cap) snprintf(err, cap, "%s", b->msg);
+            pkb_destroy(b);
+            return NULL;
+        }
+    }
     // matmul scratch: the largest need over the model's Q4_K launches at
     // n = 64 (Q/K/V and gate/up each one launch of their Q4_K matrices)
     PkMmNeed mx = {0, 0, 0, 0, 0};
@@ -1146,6 +1303,24 @@ static PkbCtx *pkb_create_ex(PkdCtx *ctx, int max_seqs, int alias, char *err, si
          !bfail(b, cudaMemsetAsync(b->mm.err, 0, 16, b->st), "cudaMemset") &&
          (alias || (!bfail(b, cudaMemsetAsync(b->kc, 0, cache, b->st), "cudaMemset") &&
                     !bfail(b, cudaMemsetAsync(b->vc, 0, cache, b->st), "cudaMemset")));
+    if (ok && page_tokens > 0) {
+        // every page free, page 0 on top
+        int *ids = (int *)malloc((size_t)n_pages * 4);
+        ok = ids != NULL;
+        for (int i = 0; ok && i < n_pages; i++) ids[i] = n_pages - 1 - i;
+        ok = ok && !bfail(b, cudaMalloc(&b->pg_d, (size_t)(3 * B) * 4), "cudaMalloc") &&
+             !bfail(b, cudaMallocHost(&b->pg_h, (size_t)(3 * B) * 4), "cudaMallocHost") &&
+             !bfail(b, cudaMalloc(&b->table, (size_t)max_seqs * b->blocks * 4), "cudaMalloc") &&
+             !bfail(b, cudaMalloc(&b->free_pages, (size_t)n_pages * 4), "cudaMalloc") &&
+             !bfail(b, cudaMalloc(&b->n_free, 16), "cudaMalloc") &&
+             !bfail(b, cudaMalloc(&b->rows, ((size_t)3 * b->row_cap + B + 1) * 4), "cudaMalloc") &&
+             !bfail(b, cudaMalloc(&b->kv_stage, (size_t)2 * KV_STAGE * kvd * 4), "cudaMalloc") &&
+             !bfail(b, cudaMemcpyAsync(b->free_pages, ids, (size_t)n_pages * 4, cudaMemcpyHostToDevice, b->st), "pages") &&
+             !bfail(b, cudaMemcpyAsync(b->n_free, &n_pages, 4, cudaMemcpyHostToDevice, b->st), "pages") &&
+             !bfail(b, cudaMemsetAsync(b->table, 0xFF, (size_t)max_seqs * b->blocks * 4, b->st), "cudaMemset") &&
+             !bfail(b, cudaStreamSynchronize(b->st), "pages");
+        free(ids);
+    }
 #define PKB_ATTR(T)                                                                                           \
     ok = ok && !bfail(b, cudaFuncSetAttribute(bt::mv_tile_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, \
                                               bt::mv_smem<T>()),                                              \
@@ -1195,9 +1370,39 @@ extern "C" int pkb_step(PkbCtx *b, const int *tokens, const int *pos, const int 
 {
     const int B = bt::BMAX;
     cudaSetDevice(b->device);
-    memcpy(b->io_h, tokens, (size_t)n * 4);
-    memcpy(b->io_h + B, pos, (size_t)n * 4);
-    memcpy(b->io_h + 2 * B, seq_ids, (size_t)n * 4);
+    // order[i]: the row in place i. A paged step takes its rows as the map
+    // makes them, sequence after sequence with ascending positions.
+    int order[bt::BMAX];
+    for (int i = 0; i < n; i++) order[i] = i;
+    if (b->paged) {
+        for (int i = 1; i < n; i++) {
+            const int r = order[i];
+            int j = i;
+            for (; j > 0; j--) {
+                const int q = order[j - 1];
+                if (seq_ids[q] < seq_ids[r] || (seq_ids[q] == seq_ids[r] && pos[q] < pos[r])) break;
+                order[j] = q;
+            }
+            order[j] = r;
+        }
+        int need = 0;
+        for (int s = 0; s < b->max_seqs; s++) b->pg_h[s] = b->pg_h[B + s] = b->pg_h[2 * B + s] = b->len[s];
+        for (int i = 0; i < n; i++) {
+            const int r = order[i], s = seq_ids[r];
+            if (i == 0 || seq_ids[order[i - 1]] != s) b->pg_h[B + s] = pos[r];
+            b->pg_h[2 * B + s] = pos[r] + 1;
+        }
+        for (int s = 0; s < b->max_seqs; s++) need += pages_for(b, b->pg_h[2 * B + s]) - pages_for(b, b->len[s]);
+        if (need > pages_left(b)) {
+            snprintf(b->msg, sizeof(b->msg), "Not enough free pages: %d needed, %d left.", need, pages_left(b));
+            return 0;
+        }
+    }
+    for (int i = 0; i < n; i++) {
+        b->io_h[i] = tokens[order[i]];
+        b->io_h[B + i] = pos[order[i]];
+        b->io_h[2 * B + i] = seq_ids[order[i]];
+    }
     // a tensor-parallel rank assembles the full logits only when asked
     // (every rank of the group must ask alike: the exchanges are collective)
     const int wl = b->world > 1 && logits != NULL ? 1 : 0;
@@ -1206,6 +1411,7 @@ extern "C" int pkb_step(PkbCtx *b, const int *tokens, const int *pos, const int 
         cudaGetLastError();
         if (bfail(b, cudaStreamBeginCapture(b->st, cudaStreamCaptureModeThreadLocal), "capture")) return 0;
         cudaMemcpyAsync(b->io_d, b->io_h, (size_t)(3 * B) * 4, cudaMemcpyHostToDevice, b->st);
+        if (b->paged) cudaMemcpyAsync(b->pg_d, b->pg_h, (size_t)(3 * B) * 4, cudaMemcpyHostToDevice, b->st);
         const int ok = enqueue_step(b, n, wl);
         cudaGraph_t g = NULL;
         const cudaError_t e = cudaStreamEndCapture(b->st, &g);
@@ -1226,7 +1432,23 @@ extern "C" int pkb_step(PkbCtx *b, const int *tokens, const int *pos, const int 
                  b->io_h[4 * B]);
         return 0;
     }
-    memcpy(next, b->io_h + 3 * B, (size_t)n * 4);
+    if (b->paged) {
+        for (int s = 0; s < b->max_seqs; s++) b->len[s] = b->pg_h[2 * B + s];
+        if (b->io_h[4 * B + 1] != 0) {
+            snprintf(b->msg, sizeof(b->msg), "The paged cache reported an error (error word %d).", b->io_h[4 * B + 1]);
+            kv_paged_error(b->paged);  // clears it
+            return 0;
+        }
+    }
+    for (int i = 0; i < n; i++) next[order[i]] = b->io_h[3 * B + i];
+    if (b->paged) {
+        const size_t row = (size_t)b->m.vocab_size;
+        for (int i = 0; logits != NULL && i < n; i++)
+            if (bfail(b, cudaMemcpyAsync(logits + order[i] * row, b->logits + i * row, row * 4, cudaMemcpyDeviceToHost, b->st),
+                      "logits copy"))
+                return 0;
+        return logits == NULL || !bfail(b, cudaStreamSynchronize(b->st), "logits copy");
+    }
     if (logits != NULL &&
         bfail(b, cudaMemcpy(logits, wl ? b->logits_full : b->logits, (size_t)n * b->m.vocab_size * 4,
                             cudaMemcpyDeviceToHost),
@@ -1252,10 +1474,13 @@ extern "C" void pkb_destroy(PkbCtx *b)
     }
     void *dev[] = {b->kv_alias ? nullptr : b->kc, b->kv_alias ? nullptr : b->vc, b->x, b->xn, b->tmp, b->q, b->att,
                    b->k, b->v, b->g, b->u, b->logits, b->part, b->io_d, b->tag0, b->logits_full,
-                   b->mm.xs, b->mm.x2s, b->mm.xinv, b->mm.ypart, b->mm.arrived, b->mm.err};
+                   b->mm.xs, b->mm.x2s, b->mm.xinv, b->mm.ypart, b->mm.arrived, b->mm.err,
+                   b->pg_d, b->table, b->free_pages, b->n_free, b->rows, b->kv_stage};
     for (void *p : dev)
         if (p) cudaFree(p);
     if (b->io_h) cudaFreeHost(b->io_h);
+    if (b->pg_h) cudaFreeHost(b->pg_h);
+    kv_paged_close(b->paged);
     if (b->ev_fork) cudaEventDestroy(b->ev_fork);
     if (b->ev_join) cudaEventDestroy(b->ev_join);
     if (b->side) cudaStreamDestroy(b->side);

@@ -145,11 +145,23 @@ PkbCtx *pkb_create(PkdCtx *ctx, int max_seqs, char *err, size_t cap);
  * layout of sequence 0 of a batched cache): prompt chunks run through the
  * batched step and land where engine_forward reads them. */
 PkbCtx *pkb_create_prefill(PkdCtx *ctx, char *err, size_t cap);
+
+/* A batched state whose sequences share a pool of n_pages pages of
+ * page_tokens tokens per layer (kv_paged.h) instead of holding a whole
+ * context each. Single GPU. */
+PkbCtx *pkb_create_paged(PkdCtx *ctx, int max_seqs, int page_tokens, int n_pages, char *err, size_t cap);
+
+/* Paged state: give sequence seq's pages back (0 on a device error), and the
+ * pages that no sequence holds (-1 for a state that is not paged). */
+int pkb_release(PkbCtx *b, int seq);
+int pkb_free_pages(const PkbCtx *b);
 void pkb_destroy(PkbCtx *b);
 
 /* Sequence seq_ids[i] takes tokens[i] at position pos[i], i < n. next[i]
  * receives the greedy token (-1 when a logit is not finite); logits (n x
- * vocab floats, host) when not NULL. Arguments are checked by the caller.
+ * vocab floats, host) when not NULL. Arguments are checked by the caller; a
+ * paged state's rows of one sequence are consecutive positions, and the
+ * sequence ends with the last of them afterwards.
  * Returns 1, or 0 on a device error (message in pkb_error). */
 int pkb_step(PkbCtx *b, const int *tokens, const int *pos, const int *seq_ids, int n, int *next, float *logits);
 const char *pkb_error(const PkbCtx *b);

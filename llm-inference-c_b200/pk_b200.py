@@ -29,7 +29,8 @@ EXPORTS = [
     "engine_is_stop_token", "engine_open_device", "engine_forward_greedy", "engine_last_error",
     "engine_weight_bytes", "engine_generate_greedy", "engine_trace", "engine_launches_per_step",
     "engine_tp_plan", "engine_open_tp", "engine_tp_handle", "engine_tp_connect",
-    "engine_batch_open", "engine_forward_batch", "engine_kv_write", "engine_prefill",
+    "engine_batch_open", "engine_batch_open_paged", "engine_batch_release", "engine_batch_free_pages",
+    "engine_forward_batch", "engine_kv_write", "engine_prefill",
     "gguf_cuda_matvec", "gguf_cuda_dequantize_rows", "gguf_cuda_fp16_table", "gguf_cuda_matvec_noalloc",
     "gguf_cuda_matvec_error", "gguf_cuda_matvec_noalloc_error",
     "gguf_cuda_matmul", "gguf_cuda_matmul_plan", "gguf_cuda_matmul_error",
@@ -151,6 +152,13 @@ def lib(path=LIB_PATH):
     L.engine_tp_connect.argtypes = [_P, _P, ctypes.c_char_p, ctypes.c_size_t]
     L.engine_batch_open.restype = ctypes.c_int
     L.engine_batch_open.argtypes = [_P, ctypes.c_int, ctypes.c_char_p, ctypes.c_size_t]
+    L.engine_batch_open_paged.restype = ctypes.c_int
+    L.engine_batch_open_paged.argtypes = [_P, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_char_p,
+                                          ctypes.c_size_t]
+    L.engine_batch_release.restype = ctypes.c_int
+    L.engine_batch_release.argtypes = [_P, ctypes.c_int]
+    L.engine_batch_free_pages.restype = ctypes.c_int
+    L.engine_batch_free_pages.argtypes = [_P]
     L.engine_forward_batch.restype = ctypes.c_int
     L.engine_forward_batch.argtypes = [_P, _P, _P, _P, ctypes.c_int, _P, _P]
     L.engine_prefill.restype = ctypes.c_int
@@ -253,6 +261,19 @@ class Engine:
         err = ctypes.create_string_buffer(512)
         if lib().engine_batch_open(self.h, max_seqs, err, 512) != 1:
             raise RuntimeError("engine_batch_open failed: " + err.value.decode())
+
+    def batch_open_paged(self, max_seqs, page_tokens, n_pages):
+        """engine_batch_open_paged: max_seqs sequences over one pool of pages."""
+        err = ctypes.create_string_buffer(512)
+        if lib().engine_batch_open_paged(self.h, max_seqs, page_tokens, n_pages, err, 512) != 1:
+            raise RuntimeError("engine_batch_open_paged failed: " + err.value.decode())
+
+    def batch_release(self, seq):
+        """engine_batch_release: the sequence starts over; its pages are free."""
+        return lib().engine_batch_release(self.h, seq) == 1
+
+    def batch_free_pages(self):
+        return lib().engine_batch_free_pages(self.h)
 
     def forward_batch(self, tokens, pos, seq_ids, logits=False):
         """engine_forward_batch: (greedy tokens, n x vocab logits or None);

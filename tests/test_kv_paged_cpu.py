@@ -144,3 +144,11 @@ def test_no_device_fails_cleanly():
         pytest.skip("a device is present")
     with pytest.raises(RuntimeError, match="CUDA"):
         handle(device=0)
+
+
+def test_engine_paged_calls_without_a_model():
+    L = pk_b200.lib()
+    err = ctypes.create_string_buffer(64)
+    assert L.engine_batch_open_paged(None, 4, 16, 8, err, 64) == 0 and err.value == b"No model."
+    assert L.engine_batch_release(None, 0) == 0
+    assert L.engine_batch_free_pages(None) == -1
