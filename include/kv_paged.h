@@ -83,6 +83,7 @@ const char *kv_paged_last_error(const KvPaged *kv);
                                   position past its row (its tokens end at the row's last) */
 #define KV_PAGED_TOO_MUCH 32   /* attend: rows x KV heads x tokens past what one call takes (16 TB of cache):
                                   no output was written */
+#define KV_PAGED_TIMEOUT 64    /* attend: a copy from the pools did not arrive in about 2 s: outputs are invalid */
 int kv_paged_error(KvPaged *kv);
 
 /*

@@ -1,6 +1,8 @@
 // kv_paged.cu - the paged key-value cache of include/kv_paged.h: block
 // tables and slot maps (map_kernel), append with rotary positions
 // (append_kernel) and attention of single new tokens (attend_kernel).
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <new>
@@ -375,29 +377,45 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
 // All items' tokens, cut into chunks, are shared out evenly over all resident
 // CTAs, whatever the rows' lengths. A warp takes every WARPS-th tile of a
 // chunk and waits for no other before an item's end: its ring of STAGES tiles
-// (keys and values, about 9 KB each) is filled by 16-byte async copies over
-// the ends of items, and the pages of the tile after them are looked up
-// meanwhile. Items that lie in one CTA's share are written at once; of the
-// others each CTA leaves its part in the scratch, and the last to arrive
-// joins them, in their order. Tokens that a row may not see are zero-filled,
-// never read.
+// (keys and values, 8 KB each) is filled over the ends of items, and the
+// pages of the tile after them are looked up meanwhile. Items that lie in
+// one CTA's share are written at once; of the others each CTA leaves its
+// part in the scratch, and the last to arrive joins them, in their order.
+//
+// Where pages are whole multiples of 8 tokens, tensor maps over the pools
+// bring a tile in boxes of 128 bytes by 8 to 32 tokens (BOXES), a few
+// instructions a tile; else each lane copies 16 bytes at a time. Both lay a
+// box's 16-byte pieces out as the maps' 128-byte swizzle does (piece c of
+// token r at c ^ (r mod 8)), so that reads of eight tokens meet no bank twice.
+// Tokens that a row may not see do not count: copies leave them out or, in
+// the box that a row ends in, their values are zeroed before use.
 constexpr int ATT_HEADS = 8;
 constexpr float ATT_JOIN = 0.2f;  // the cost of a part over that of a chunk
 
-template <typename KV, int HSP>
+template <typename KV, int HSP, bool BOXES>
 struct Geo {
     static constexpr bool HALF = sizeof(KV) == 2;
     static constexpr int TILE = HALF ? (HSP == 64 ? 32 : 16) : (HSP == 64 ? 16 : 8);  // tokens
     static constexpr int WARPS = 4;
     static constexpr int STAGES = HSP == 256 ? 1 : 2;
-    static constexpr int CTAS = HSP == 256 ? 2 : 3;  // per SM, as shared memory allows
+    // CTAs an SM: three, as shared memory allows (two of 256 channels). With
+    // 128 half channels in boxes two are better: they leave 130 KB an SM in
+    // flight instead of 200, and SMs then get more equal shares of the
+    // memory's bandwidth (64 rows of up to 8192 tokens 188 instead of 193 us,
+    // 16 rows of 2030, 32 KV heads 90 instead of 95, though 128 rows of up to
+    // 200 tokens 29 instead of 25). Where a tile costs more instructions, a
+    // float one three times as many, 12 warps win: 16 rows of 1030 tokens,
+    // 32 KV heads (float) 96 instead of 108 us.
+    static constexpr int CTAS = HSP == 256 || (HALF && HSP == 128 && BOXES) ? 2 : 3;
     static constexpr int CHUNK = WARPS * TILE;       // tokens: the unit in which work is shared out
-    static constexpr int ROW = HSP * (int)sizeof(KV) + 16;  // bytes; 16 past a multiple of 128: no bank conflicts
-    static constexpr int STAGE = 2 * TILE * ROW;
+    static constexpr int WIDE = HSP * (int)sizeof(KV) / 128;  // boxes side by side
+    static constexpr int BOX = TILE * 128;                    // bytes of a column of boxes
+    static constexpr int SIDE = WIDE * BOX;                   // of a tile's keys; its values follow
+    static constexpr int STAGE = 2 * SIDE;
     static constexpr int RING = STAGES * STAGE;
     static constexpr int SEGS = HSP * (int)sizeof(KV) / 16;  // 16-byte pieces of a token's head
     static constexpr int KS = HALF ? HSP / 16 : HSP / 8;     // steps of a score's product
-    static constexpr int SMEM = WARPS * RING + KS * 512;     // rings, then q as the products' left operand
+    static constexpr int SMEM = 1024 + WARPS * RING + KS * 512;  // rings on 1024 bytes, then q as the left operand
     static constexpr int OROW = HSP + 8;                     // floats from a head to the next of sums that wait to be joined
     static constexpr int PART = ATT_HEADS * OROW;            // floats of a part
     static_assert(PART * 4 <= STAGE, "a warp's sums fit a stage");
@@ -409,9 +427,11 @@ struct AttendArgs {
     const int *table, *row_request, *row_pos;
     int n, n_requests, heads, kv_heads, hs;
     int groups, group_heads;  // a KV head's items, and the query heads of each
+    Div by_groups, by_f4;     // f4: head size / 4
     float scale;
     float *out;
     uint64_t q_stride;
+    int box_shift;  // BOXES: log2 of a box's tokens
     Cache c;
     float *part;        // [2 * grid][ATT_HEADS][OROW]: a head's sums, then its maximum and weight at HSP
     unsigned *arrived;  // [grid]: parts of the item that begins in CTA b and ends in another; wraps to 0 by itself
@@ -459,6 +479,12 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t &hi, uint32_t &lo)
     hi = (__float_as_uint(x) + 0x1000u) & 0xFFFFE000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
+// The same of a key, whose products only enter a score: x itself is the upper
+// part (the product cuts it off), and up to 2^-21 of x is lost.
+__device__ __forceinline__ uint32_t rest_tf32(uint32_t x)
+{
+    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xFFFFE000u));
+}
 // (x, y) = hi + lo, each a pair of halves.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32_t &lo)
 {
@@ -476,6 +502,21 @@ __device__ __forceinline__ void add_tile(float (&o)[2], const float (&x)[4], flo
 {
     o[0] = fmaf(o[0], f, x[0] + x[2]);
     o[1] = fmaf(o[1], f, x[1] + x[3]);
+}
+// Waits until the barrier's phase is over: false when it is not after about
+// two seconds.
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t phase)
+{
+    const long long t0 = clock64();
+    while (true) {
+        uint32_t done;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done)
+                     : "r"(bar), "r"(phase)
+                     : "memory");
+        if (__all_sync(0xFFFFFFFFu, done)) return true;
+        if (__any_sync(0xFFFFFFFFu, clock64() - t0 > 4000000000ll)) return false;
+    }
 }
 // 2^(x - top), for a part's maximum x and the maximum of all parts.
 __device__ __forceinline__ float weight_of(float x, float top)
@@ -552,14 +593,17 @@ struct Part {
     int r, h0, heads, b0, parts;  // the item's first CTA, and how many hold it (0: no such part)
 };
 
-template <typename KV, int HSP>
-__global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) attend_kernel(const AttendArgs a)
+template <typename KV, int HSP, bool BOXES>
+__global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, BOXES>::CTAS)
+    attend_kernel(const AttendArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map)
 {
-    using G = Geo<KV, HSP>;
+    using G = Geo<KV, HSP, BOXES>;
     constexpr int TILE = G::TILE, CHUNK = G::CHUNK, W = G::WARPS, NT = TILE / 8, DT = HSP / 8, KS = G::KS;
     constexpr int JT = (ATT_HEADS * HSP / 4 + 32 * W - 1) / (32 * W);  // pieces of 4 channels of all heads, per thread
     constexpr int HW = (ATT_HEADS + W - 1) / W;  // heads of a warp
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - ((uint32_t)__cvta_generic_to_shared(smem_raw) & 1023u)) & 1023u);
+    __shared__ __align__(8) uint64_t bars[W][G::STAGES];  // BOXES: a tile's copies have arrived
     __shared__ float head_unit[ATT_HEADS];           // score = product * unit
     __shared__ float wm[ATT_HEADS][W], wl[ATT_HEADS][W];  // warps' maxima and weights
     __shared__ const float *wo[W];                   // where a warp left its sums
@@ -573,7 +617,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
     const int items = a.kv_heads * a.groups, b = blockIdx.x;
     const int group = a.heads / a.kv_heads, F4 = a.hs >> 2;
     auto heads_of = [&](int it, int &h0, int &H) {
-        const int kvh = it / a.groups, grp = it - kvh * a.groups;
+        const int kvh = div_by(a.by_groups, it), grp = it - kvh * a.groups;
         h0 = kvh * group + grp * a.group_heads;
         H = min(a.group_heads, group - grp * a.group_heads);
     };
@@ -661,12 +705,14 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
         l_tok = lp.c * CHUNK + warp * TILE;
         l_stop = lp.stop();
         l_table = a.table + (size_t)lp.req * a.c.max_blocks;
-        l_head = (uint32_t)(lp.it / a.groups) * a.c.head_units;
+        l_head = (uint32_t)div_by(a.by_groups, lp.it);
     };
-    uint32_t nx_at = 0;  // where the next tile's token `lane` lies, in 16 bytes
-    bool nx_ok = false, nx_any = false;
-    int nx_page = -1, nx_place = 0;
-    // looks up the pages of the next tile: token `lane` of it
+    // the next tile: its tokens that count, and the page and place of its
+    // token (BOXES: box) `lane`
+    bool nx_any = false;
+    int nx_count = 0, nx_page = -1, nx_place = 0;
+    uint32_t nx_head = 0;
+    const int unit_shift = BOXES ? a.box_shift : 0;
     auto look = [&]() {
         while (l_more && l_tok >= l_stop) {
             lp.next(a, items);
@@ -677,49 +723,85 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
             }
         }
         nx_any = l_more;
-        nx_ok = false;
         if (!l_more) return;
-        const int tok = l_tok + lane;
-        if (lane < TILE && tok < l_stop) {
-            const int blk = div_by(a.c.page, tok);
+        nx_count = min(TILE, l_stop - l_tok);
+        const int off = lane << unit_shift;
+        nx_page = -1;
+        if (off < nx_count) {
+            const int tok = l_tok + off, blk = div_by(a.c.page, tok);
             nx_place = tok - blk * (int)a.c.page.d;
             nx_page = l_table[blk];
-            nx_ok = true;
         }
-        nx_at = l_head;
+        nx_head = l_head;
         l_tok += CHUNK;
     };
+    const uint32_t bar_s = (uint32_t)__cvta_generic_to_shared(&bars[warp][0]);
+    uint32_t phases = 0;   // of the warp's barriers, a bit a stage
+    bool written = false;  // the slot that is filled next was written by this warp
+    if (BOXES) {
+        if (lane < G::STAGES) asm volatile("mbarrier.init.shared.b64 [%0], 1;" ::"r"(bar_s + 8 * lane) : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+    }
     auto issue = [&](int slot) {
         if (nx_any) {
-            uint32_t at = nx_at;
-            const int page = nx_page, place = nx_place;
-            bool ok = nx_ok;
+            const int page = nx_page, place = nx_place, count = nx_count;
+            const uint32_t head = nx_head;
             look();  // the tile after this one: its page numbers are there when it is issued
-            if (ok && (page < 0 || page >= a.c.n_pages)) {
-                atomicOr(a.err, KV_PAGED_BAD_PAGE);
-                ok = false;
-            }
-            const uint32_t mask = __ballot_sync(0xFFFFFFFFu, ok);
-            if (lane == 0) masks[warp][slot] = mask;
-            if (ok) at += (uint32_t)page * a.c.page_units + (uint32_t)place * a.c.token_units;
+            const bool asked = (lane << unit_shift) < count;
+            const bool ok = asked && page >= 0 && page < a.c.n_pages;
+            if (asked && !ok) atomicOr(a.err, KV_PAGED_BAD_PAGE);
+            const uint32_t there = __ballot_sync(0xFFFFFFFFu, ok);  // tokens (BOXES: boxes) that are copied
             const uint32_t dst0 = ring_s + slot * G::STAGE;
+            if (BOXES) {
+                const uint32_t mask =
+                    __ballot_sync(0xFFFFFFFFu, lane < count && ((there >> (lane >> unit_shift)) & 1u) != 0u);
+                const uint32_t bar = bar_s + 8 * slot;
+                if (written) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    written = false;
+                }
+                if (lane == 0) {
+                    masks[warp][slot] = mask;
+                    const uint32_t bytes = (uint32_t)__popc(there) * 2u * G::WIDE * 128u << unit_shift;
+                    asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+                }
+                __syncwarp();
+                // a lane a box: of keys or values, of the boxes side by side, of the tile's tokens
+                const int sub = lane / (2 * G::WIDE), col = (lane >> 1) % G::WIDE;
+                const int bp = __shfl_sync(0xFFFFFFFFu, page, sub), bl = __shfl_sync(0xFFFFFFFFu, place, sub);
+                if ((there >> sub) & 1u) {
+                    const uint32_t dst = dst0 + (lane & 1) * G::SIDE + col * G::BOX + (uint32_t)(sub * 128 << unit_shift);
+                    const CUtensorMap *map = (lane & 1) ? &v_map : &k_map;
+                    asm volatile(
+                        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                        "%4, %5}], [%6];" ::"r"(dst),
+                        "l"(map), "r"(col * (128 / (int)sizeof(KV))), "r"(head), "r"(bl), "r"(bp), "r"(bar)
+                        : "memory");
+                }
+            } else {
+                if (lane == 0) masks[warp][slot] = there;
+                uint32_t at = head * a.c.head_units;
+                if (ok) at += (uint32_t)page * a.c.page_units + (uint32_t)place * a.c.token_units;
+                constexpr int SEGS = 8 * G::WIDE;  // 16-byte pieces of a token's head
 #pragma unroll
-            for (int i = 0; i < TILE * G::SEGS / 32; i++) {
-                const int idx = lane + 32 * i, key = idx / G::SEGS, seg = idx % G::SEGS;
-                const uint32_t from = __shfl_sync(0xFFFFFFFFu, at, key);
-                const bool in = ((mask >> key) & 1u) && seg < segs;
-                const int bytes = in ? 16 : 0;
-                const uint64_t e = in ? (uint64_t)(from + seg) * 16 : 0;
-                const uint32_t dst = dst0 + key * G::ROW + seg * 16;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
-                             "l"(static_cast<const uint8_t *>(a.k_pool) + e), "r"(bytes)
-                             : "memory");
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + TILE * G::ROW),
-                             "l"(static_cast<const uint8_t *>(a.v_pool) + e), "r"(bytes)
-                             : "memory");
+                for (int i = 0; i < TILE * SEGS / 32; i++) {
+                    const int idx = lane + 32 * i, key = idx / SEGS, seg = idx % SEGS;
+                    const uint32_t from = __shfl_sync(0xFFFFFFFFu, at, key);
+                    const bool in = ((there >> key) & 1u) && seg < segs;
+                    const int bytes = in ? 16 : 0;
+                    const uint64_t e = in ? (uint64_t)(from + seg) * 16 : 0;
+                    const uint32_t dst = dst0 + (seg >> 3) * G::BOX + key * 128 + (((seg ^ key) & 7) << 4);
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
+                                 "l"(static_cast<const uint8_t *>(a.k_pool) + e), "r"(bytes)
+                                 : "memory");
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + G::SIDE),
+                                 "l"(static_cast<const uint8_t *>(a.v_pool) + e), "r"(bytes)
+                                 : "memory");
+                }
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (!BOXES) asm volatile("cp.async.commit_group;" ::: "memory");
     };
 
     // ---- q: head h by warp h mod W; loaded an item ahead ----
@@ -805,6 +887,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
     int slot = 0, fill = G::STAGES;  // tiles to ask for before the next is used
     int tok = cp.c * CHUNK + warp * TILE, stop = cp.stop();
     bool hold = false;  // this warp's last slot waits for the item's end
+    bool lost = false;  // a tile did not arrive
     bool fresh = true, used = false;  // q is to be made; this warp has had a tile of the item
     float o[DT][2], m = -INFINITY, l = 0.0f, unit = 1.0f;
 #pragma unroll
@@ -835,16 +918,37 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
         if (tok < stop) {
             tok += CHUNK;
             used = true;
-            asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 1) : "memory");
+            uint32_t mask = 0u;
+            if (BOXES) {
+                if (!lost && !arrived(bar_s + 8 * slot, (phases >> slot) & 1u)) {
+                    // nothing more is asked for, and what is left counts for nothing
+                    atomicOr(a.err, KV_PAGED_TIMEOUT);
+                    lost = true;
+                    l_more = nx_any = false;
+                }
+                phases ^= 1u << slot;
+            } else {
+                asm volatile("cp.async.wait_group %0;" ::"n"(G::STAGES - 1) : "memory");
+            }
             __syncwarp();
-            const uint32_t mask = masks[warp][slot];
-            const uint32_t ks_s = ring_s + slot * G::STAGE, vs_s = ks_s + TILE * G::ROW;
+            if (!lost) mask = masks[warp][slot];
+            const uint32_t ks_s = ring_s + slot * G::STAGE, vs_s = ks_s + G::SIDE;
+            if (BOXES && mask != (uint32_t)((1ull << TILE) - 1)) {
+                // tokens that do not count: what they hold must not meet p = 0
+                for (int i = lane; i < TILE * 8 * G::WIDE; i += 32) {
+                    const int key = (i >> 3) % TILE;
+                    if (!((mask >> key) & 1u))
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs_s + 16 * i), "r"(0u) : "memory");
+                }
+                written = true;
+                __syncwarp();
+            }
             if (mask != 0u) {
                 float s[NT][4];
 #pragma unroll
                 for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
                 if (G::HALF) {
-                    const uint32_t at = ks_s + ((lane >> 4) * 8 + (lane & 7)) * G::ROW + ((lane >> 3) & 1) * 16;
+                    const uint32_t at = ks_s + ((lane >> 4) * 8 + (lane & 7)) * 128, piece = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++) {
                         uint32_t qa[4];
@@ -852,7 +956,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
 #pragma unroll
                         for (int j = 0; j < NT / 2; j++) {
                             uint32_t kb[4];
-                            ldmatrix4(kb, at + 16 * j * G::ROW + ks * 32);
+                            ldmatrix4(kb, at + (ks / 4) * G::BOX + 16 * j * 128 + (piece ^ ((ks & 3) << 5)));
                             mma_f16(s[2 * j], qa, kb[0], kb[1]);
                             mma_f16(s[2 * j + 1], qa, kb[2], kb[3]);
                         }
@@ -861,7 +965,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
                     float s2[NT][4];  // the lower parts' products, a second chain
 #pragma unroll
                     for (int j = 0; j < NT; j++) s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.0f;
-                    const uint32_t at = ks_s + (lane & 7) * G::ROW + (lane >> 3) * 16;
+                    const uint32_t at = ks_s + (lane & 7) * 128, piece = ((lane >> 3) ^ (lane & 7)) << 4;
 #pragma unroll
                     for (int ks = 0; ks < KS / 2; ks++) {
                         uint32_t qa[4], qb[4];
@@ -869,14 +973,12 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
                         q_step(2 * ks + 1, qb);
 #pragma unroll
                         for (int j = 0; j < NT; j++) {
-                            uint32_t kb[4], hi[4], lo[4];
-                            ldmatrix4(kb, at + 8 * j * G::ROW + ks * 64);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) split_tf32(__uint_as_float(kb[i]), hi[i], lo[i]);
-                            mma_tf32(s[j], qa, hi[0], hi[1]);
-                            mma_tf32(s2[j], qa, lo[0], lo[1]);
-                            mma_tf32(s[j], qb, hi[2], hi[3]);
-                            mma_tf32(s2[j], qb, lo[2], lo[3]);
+                            uint32_t kb[4];
+                            ldmatrix4(kb, at + (ks / 2) * G::BOX + 8 * j * 128 + (piece ^ ((ks & 1) << 6)));
+                            mma_tf32(s[j], qa, kb[0], kb[1]);
+                            mma_tf32(s2[j], qa, rest_tf32(kb[0]), rest_tf32(kb[1]));
+                            mma_tf32(s[j], qb, kb[2], kb[3]);
+                            mma_tf32(s2[j], qb, rest_tf32(kb[2]), rest_tf32(kb[3]));
                         }
                     }
 #pragma unroll
@@ -917,11 +1019,12 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
                         uint32_t pa[4];
                         split_f16(p[2 * kb][0], p[2 * kb][1], pa[0], pa[1]);
                         split_f16(p[2 * kb + 1][0], p[2 * kb + 1][1], pa[2], pa[3]);
-                        const uint32_t at = vs_s + (16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7)) * G::ROW + (lane >> 4) * 16;
+                        const uint32_t at = vs_s + (16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+                        const uint32_t piece = ((lane >> 4) ^ (lane & 7)) << 4;
 #pragma unroll
                         for (int i = 0; i < DT / 2; i++) {
                             uint32_t vb[4];
-                            ldmatrix4_t(vb, at + i * 32);
+                            ldmatrix4_t(vb, at + (i / 4) * G::BOX + (piece ^ ((i & 3) << 5)));
                             float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                             mma_f16(x, pa, vb[0], vb[1]);
                             mma_f16(y, pa, vb[2], vb[3]);
@@ -937,12 +1040,11 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
                         uint32_t pa[4];
                         split_tf32(p[kb][0], pa[0], pa[1]);
                         split_tf32(p[kb][1], pa[2], pa[3]);
-                        const float *v0 = reinterpret_cast<const float *>(
-                            ring + slot * G::STAGE + (TILE + 8 * kb + 2 * t4) * G::ROW + g * 16);
+                        const uint8_t *v0 = ring + slot * G::STAGE + G::SIDE + (8 * kb + 2 * t4) * 128;
 #pragma unroll
                         for (int c = 0; c < HSP / 32; c++) {
-                            const float4 x = *reinterpret_cast<const float4 *>(v0 + 32 * c);
-                            const float4 y = *reinterpret_cast<const float4 *>(v0 + G::ROW / 4 + 32 * c);
+                            const float4 x = *reinterpret_cast<const float4 *>(v0 + c * G::BOX + ((g ^ (2 * t4)) << 4));
+                            const float4 y = *reinterpret_cast<const float4 *>(v0 + c * G::BOX + 128 + ((g ^ (2 * t4 + 1)) << 4));
                             const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
@@ -963,7 +1065,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
                 fill = 1;
                 continue;
             }
-            hold = true;  // the last tile's slot is filled again after the item's end
+            hold = written = true;  // the last tile's slot is filled again after the item's end
         }
         // ---- the item's end: the warps' sums, each in the slot of its last tile ----
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
@@ -999,7 +1101,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
         float *part = a.part + (size_t)(2 * b + side) * G::PART;
         float *out = a.out + ((size_t)cp.r * a.heads + h0) * a.hs;
         for (int i = tid; i < H * F4; i += 32 * W) {
-            const int h = i / F4, d = 4 * (i - h * F4);
+            const int h = div_by(a.by_f4, i), d = 4 * (i - h * F4);
             float mt = -INFINITY, lt = 0.0f;
 #pragma unroll
             for (int w = 0; w < W; w++)
@@ -1043,7 +1145,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
 #pragma unroll
         for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!BOXES) asm volatile("cp.async.wait_all;" ::: "memory");
 
     // ---- parts: the last of an item's CTAs to arrive joins them in their order ----
     __syncthreads();
@@ -1105,7 +1207,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
             __syncthreads();
 #pragma unroll
             for (int c = 0; c < JT; c++) {
-                const int i = tid + 32 * W * c, h = i / F4, d = 4 * (i - h * F4);
+                const int i = tid + 32 * W * c, h = div_by(a.by_f4, i), d = 4 * (i - h * F4);
                 if (h >= p.heads) break;
                 const float top = jm[h];
                 const float *ph = reinterpret_cast<const float *>(smem) + h * G::OROW;
@@ -1123,7 +1225,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::CTAS) 
         }
 #pragma unroll
         for (int c = 0; c < JT; c++) {
-            const int i = tid + 32 * W * c, h = i / F4, d = 4 * (i - h * F4);
+            const int i = tid + 32 * W * c, h = div_by(a.by_f4, i), d = 4 * (i - h * F4);
             if (h >= p.heads) break;
             const float lt = jl[h], inv = lt != 0.0f ? 1.0f / lt : 0.0f;
             *reinterpret_cast<float4 *>(out + h * a.hs + d) = make_float4(s[c].x * inv, s[c].y * inv, s[c].z * inv, s[c].w * inv);
@@ -1143,6 +1245,8 @@ struct KvPaged {
     int device, sms;
     int hsp;            // attend: head size that the kernel is built for, 64, 128 or 256
     int grid;           // attend: CTAs, as many as are resident at once
+    bool boxes;         // attend: tiles come by tensor maps,
+    int box_shift;      // in boxes of 2^box_shift tokens
     uint8_t *scratch;   // device: all of the below
     int *err;           // error bits
     unsigned *map_arrived;
@@ -1224,14 +1328,52 @@ static int launched(KvPaged *kv, const char *what)
     return 0;
 }
 
-// use(kernel, threads, dynamic shared memory, floats of a part) of a handle's attention.
+// cuTensorMapEncodeTiled, from the driver through the runtime (no link against
+// the driver library). NULL where it is missing.
+static PFN_cuTensorMapEncodeTiled_v12000 encode_tiled()
+{
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p) : nullptr;
+    }();
+    return fn;
+}
+
+// The map of a pool: channels, KV heads, a page's tokens, pages; boxes of 128
+// bytes by 2^box_shift tokens. Channels past the head size read as 0.
+static bool pool_map(const KvPaged *kv, const void *pool, CUtensorMap *map)
+{
+    const KvPagedShape &s = kv->s;
+    const cuuint64_t size = s.type == 1 ? 2 : 4;
+    const cuuint64_t dims[4] = {(cuuint64_t)s.head_size, (cuuint64_t)s.n_kv_heads, (cuuint64_t)s.page_tokens,
+                                (cuuint64_t)s.n_pages};
+    // the stride of an axis with a single entry is never used, but must be a proper one
+    auto stride = [&](uint64_t entries, int count) { return count > 1 ? entries * size : (cuuint64_t)16; };
+    const cuuint64_t strides[3] = {stride(s.head_stride, s.n_kv_heads), stride(s.token_stride, s.page_tokens),
+                                   stride(s.page_stride, s.n_pages)};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, 1u << kv->box_shift, 1}, step[4] = {1, 1, 1, 1};
+    return encode_tiled()(map, s.type == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
+                          const_cast<void *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// use(kernel, threads, dynamic shared memory, floats of a part, tokens of a
+// tile) of a handle's attention.
 template <typename F>
 static auto with_attend(const KvPaged *kv, F use)
 {
     using namespace kvp;
-#define KVP_CASE(KV, HSP) use(attend_kernel<KV, HSP>, 32 * Geo<KV, HSP>::WARPS, Geo<KV, HSP>::SMEM, Geo<KV, HSP>::PART)
+#define KVP_KERNEL(KV, HSP, BOXES) \
+    use(attend_kernel<KV, HSP, BOXES>, 32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, BOXES>::SMEM, Geo<KV, HSP, BOXES>::PART, \
+        Geo<KV, HSP, BOXES>::TILE)
+#define KVP_CASE(KV, HSP) (kv->boxes ? KVP_KERNEL(KV, HSP, true) : KVP_KERNEL(KV, HSP, false))
     if (kv->s.type == 1) return kv->hsp == 64 ? KVP_CASE(__half, 64) : kv->hsp == 128 ? KVP_CASE(__half, 128) : KVP_CASE(__half, 256);
-    return kv->hsp == 64 ? KVP_CASE(float, 64) : kv->hsp == 128 ? KVP_CASE(float, 128) : KVP_CASE(float, 256);
+    return kv->hsp == 64 ? KVP_CASE(float, 64) : kv->hsp == 128 ? KVP_CASE(float, 128) : KVP_KERNEL(float, 256, false);
+#undef KVP_KERNEL
 #undef KVP_CASE
 }
 
@@ -1273,13 +1415,19 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
         OnDevice on(device);
         e = on.ok ? cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device) : cudaErrorInvalidDevice;
         size_t parts = 0;
+        // 256 floats are 16 boxes of 1 KB a tile: 122 us for 32 rows of 2000 tokens, 102 us by 16-byte copies
+        kv->boxes = s.page_tokens % 8 == 0 && !(s.type == 0 && s.head_size > 128) && encode_tiled() != nullptr;
         kv->hsp = s.head_size <= 64 ? 64 : s.head_size <= 128 ? 128 : 256;
         if (e == cudaSuccess) {
-            e = with_attend(kv, [&](auto kernel, int threads, int smem, int floats) {
+            e = with_attend(kv, [&](auto kernel, int threads, int smem, int floats, int tile) {
                 int per_sm = 0;
                 cudaError_t x = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
                 if (x == cudaSuccess) x = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem);
                 kv->grid = per_sm * kv->sms;
+                // boxes lie within a page and a tile: the largest power of two that divides both
+                for (kv->box_shift = 0; kv->boxes && (1 << kv->box_shift) < tile &&
+                                        kv->s.page_tokens % (2 << kv->box_shift) == 0;)
+                    kv->box_shift++;
                 parts = (size_t)kv->grid * 2 * floats * 4;
                 return x == cudaSuccess && per_sm < 1 ? cudaErrorInvalidConfiguration : x;
             });
@@ -1454,16 +1602,24 @@ extern "C" int kv_paged_attend(KvPaged *kv, const float *q, const void *k_pool, 
     const int group = s.n_heads / s.n_kv_heads;
     a.groups = (group + kvp::ATT_HEADS - 1) / kvp::ATT_HEADS;
     a.group_heads = (group + a.groups - 1) / a.groups;
+    a.by_groups = kvp::make_div((uint32_t)a.groups);
+    a.by_f4 = kvp::make_div((uint32_t)s.head_size / 4);
     a.scale = scale;
     a.out = out;
     a.q_stride = q_stride;
     a.c = kv->c;
+    a.box_shift = kv->box_shift;
     a.part = kv->part;
     a.arrived = kv->arrived;
     a.err = kv->err;
+    CUtensorMap k_map, v_map;
+    memset(&k_map, 0, sizeof(k_map));
+    v_map = k_map;
+    if (kv->boxes && (!pool_map(kv, k_pool, &k_map) || !pool_map(kv, v_pool, &v_map)))
+        return refuse(kv, "attend: the driver cannot map the pools.");
     cudaGetLastError();
-    with_attend(kv, [&](auto kernel, int threads, int smem, int) {
-        kernel<<<kv->grid, threads, smem, (cudaStream_t)stream>>>(a);
+    with_attend(kv, [&](auto kernel, int threads, int smem, int, int) {
+        kernel<<<kv->grid, threads, smem, (cudaStream_t)stream>>>(a, k_map, v_map);
         return cudaSuccess;
     });
     return launched(kv, "attend");
