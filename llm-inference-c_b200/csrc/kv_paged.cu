@@ -395,18 +395,15 @@ constexpr float ATT_JOIN = 0.2f;  // the cost of a part over that of a chunk
 template <typename KV, int HSP, bool BOXES>
 struct Geo {
     static constexpr bool HALF = sizeof(KV) == 2;
-    static constexpr int TILE = HALF ? (HSP == 64 ? 32 : 16) : (HSP == 64 ? 16 : 8);  // tokens
+    static constexpr int TILE = HALF ? (HSP <= 128 ? 32 : 16) : (HSP == 64 ? 16 : 8);  // tokens
     static constexpr int WARPS = 4;
-    static constexpr int STAGES = HSP == 256 ? 1 : 2;
-    // CTAs an SM: three, as shared memory allows (two of 256 channels). With
-    // 128 half channels in boxes two are better: they leave 130 KB an SM in
-    // flight instead of 200, and SMs then get more equal shares of the
-    // memory's bandwidth (64 rows of up to 8192 tokens 188 instead of 193 us,
-    // 16 rows of 2030, 32 KV heads 90 instead of 95, though 128 rows of up to
-    // 200 tokens 29 instead of 25). Where a tile costs more instructions, a
-    // float one three times as many, 12 warps win: 16 rows of 1030 tokens,
-    // 32 KV heads (float) 96 instead of 108 us.
-    static constexpr int CTAS = HSP == 256 || (HALF && HSP == 128 && BOXES) ? 2 : 3;
+    // 16 KB a warp: one tile of 128 half or 256 channels, two of the others.
+    // One of 32 tokens instead of two of 16 spreads what a tile costs beyond
+    // its products over more of them (40 rows of up to 4000 tokens, 24 heads
+    // on 2 KV heads of 80: 35 instead of 45 us; 64 rows of up to 8192 the
+    // same); twelve warps an SM cover the wait for the next.
+    static constexpr int STAGES = HSP == 256 || (HALF && HSP == 128) ? 1 : 2;
+    static constexpr int CTAS = HSP == 256 ? 2 : 3;  // per SM, as shared memory allows
     static constexpr int CHUNK = WARPS * TILE;       // tokens: the unit in which work is shared out
     static constexpr int WIDE = HSP * (int)sizeof(KV) / 128;  // boxes side by side
     static constexpr int BOX = TILE * 128;                    // bytes of a column of boxes
@@ -852,7 +849,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
 #pragma unroll
             for (int i = 0; i < HSP / 64; i++) {
                 const int d = 2 * lane + 64 * i;
-                if (G::HALF) {
+                if constexpr (G::HALF) {
                     uint32_t hi, lo;
                     split_f16(x[2 * i], x[2 * i + 1], hi, lo);
                     const int kk = d & 15;
@@ -947,7 +944,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                 float s[NT][4];
 #pragma unroll
                 for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-                if (G::HALF) {
+                if constexpr (G::HALF) {
                     const uint32_t at = ks_s + ((lane >> 4) * 8 + (lane & 7)) * 128, piece = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++) {
@@ -1013,50 +1010,59 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                         l += p[j][i];
                     }
                 }
-                if (G::HALF) {
+                if constexpr (G::HALF) {
+                    uint32_t pa[TILE / 16][4];
 #pragma unroll
                     for (int kb = 0; kb < TILE / 16; kb++) {
-                        uint32_t pa[4];
-                        split_f16(p[2 * kb][0], p[2 * kb][1], pa[0], pa[1]);
-                        split_f16(p[2 * kb + 1][0], p[2 * kb + 1][1], pa[2], pa[3]);
-                        const uint32_t at = vs_s + (16 * kb + ((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
-                        const uint32_t piece = ((lane >> 4) ^ (lane & 7)) << 4;
+                        split_f16(p[2 * kb][0], p[2 * kb][1], pa[kb][0], pa[kb][1]);
+                        split_f16(p[2 * kb + 1][0], p[2 * kb + 1][1], pa[kb][2], pa[kb][3]);
+                    }
+                    const uint32_t at = vs_s + (((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+                    const uint32_t piece = ((lane >> 4) ^ (lane & 7)) << 4;
 #pragma unroll
-                        for (int i = 0; i < DT / 2; i++) {
+                    for (int i = 0; i < DT / 2; i++) {
+                        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int kb = 0; kb < TILE / 16; kb++) {
                             uint32_t vb[4];
-                            ldmatrix4_t(vb, at + (i / 4) * G::BOX + (piece ^ ((i & 3) << 5)));
-                            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_f16(x, pa, vb[0], vb[1]);
-                            mma_f16(y, pa, vb[2], vb[3]);
-                            add_tile(o[2 * i], x, kb == 0 ? f : 1.0f);
-                            add_tile(o[2 * i + 1], y, kb == 0 ? f : 1.0f);
+                            ldmatrix4_t(vb, at + (i / 4) * G::BOX + 16 * kb * 128 + (piece ^ ((i & 3) << 5)));
+                            mma_f16(x, pa[kb], vb[0], vb[1]);
+                            mma_f16(y, pa[kb], vb[2], vb[3]);
                         }
+                        add_tile(o[2 * i], x, f);
+                        add_tile(o[2 * i + 1], y, f);
                     }
                 } else {
                     // inner index t4 stands for token 2 t4, t4 + 4 for 2 t4 + 1;
                     // column g of o[4c + i] for channel 32c + 4g + i
+                    uint32_t pa[NT][4];
 #pragma unroll
                     for (int kb = 0; kb < NT; kb++) {
-                        uint32_t pa[4];
-                        split_tf32(p[kb][0], pa[0], pa[1]);
-                        split_tf32(p[kb][1], pa[2], pa[3]);
-                        const uint8_t *v0 = ring + slot * G::STAGE + G::SIDE + (8 * kb + 2 * t4) * 128;
+                        split_tf32(p[kb][0], pa[kb][0], pa[kb][1]);
+                        split_tf32(p[kb][1], pa[kb][2], pa[kb][3]);
+                    }
+                    const uint8_t *v0 = ring + slot * G::STAGE + G::SIDE + 2 * t4 * 128;
 #pragma unroll
-                        for (int c = 0; c < HSP / 32; c++) {
-                            const float4 x = *reinterpret_cast<const float4 *>(v0 + c * G::BOX + ((g ^ (2 * t4)) << 4));
-                            const float4 y = *reinterpret_cast<const float4 *>(v0 + c * G::BOX + 128 + ((g ^ (2 * t4 + 1)) << 4));
+                    for (int c = 0; c < HSP / 32; c++) {
+                        float s4[4][4];
+#pragma unroll
+                        for (int kb = 0; kb < NT; kb++) {
+                            const uint8_t *vk = v0 + c * G::BOX + 8 * kb * 128;
+                            const float4 x = *reinterpret_cast<const float4 *>(vk + ((g ^ (2 * t4)) << 4));
+                            const float4 y = *reinterpret_cast<const float4 *>(vk + 128 + ((g ^ (2 * t4 + 1)) << 4));
                             const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
                                 uint32_t xh, xl, yh, yl;
                                 split_tf32(xs[i], xh, xl);
                                 split_tf32(ys[i], yh, yl);
-                                float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                mma_tf32(s4, pa, xl, yl);
-                                mma_tf32(s4, pa, xh, yh);
-                                add_tile(o[4 * c + i], s4, kb == 0 ? f : 1.0f);
+                                if (kb == 0) s4[i][0] = s4[i][1] = s4[i][2] = s4[i][3] = 0.0f;
+                                mma_tf32(s4[i], pa[kb], xl, yl);
+                                mma_tf32(s4[i], pa[kb], xh, yh);
                             }
                         }
+#pragma unroll
+                        for (int i = 0; i < 4; i++) add_tile(o[4 * c + i], s4[i], f);
                     }
                 }
             }
@@ -1075,7 +1081,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
             float *dst = mine_o + g * G::OROW;
 #pragma unroll
             for (int i = 0; i < DT; i += G::HALF ? 1 : 4) {
-                if (G::HALF) {
+                if constexpr (G::HALF) {
                     *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t4) = make_float2(o[i][0], o[i][1]);
                 } else {
 #pragma unroll
