@@ -81,7 +81,7 @@ const char *kv_paged_last_error(const KvPaged *kv);
 #define KV_PAGED_BAD_ROW 16    /* append: a slot past the pool or a position past the rotary table (row
                                   passed over); attend: a request past the table (row passed over) or a
                                   position past its row (its tokens end at the row's last) */
-#define KV_PAGED_TOO_MUCH 32   /* attend: rows x KV heads x tokens past what one call takes (16 TB of cache):
+#define KV_PAGED_TOO_MUCH 32   /* attend: rows x KV heads x tokens past what one call takes (64 TB of cache):
                                   no output was written */
 #define KV_PAGED_TIMEOUT 64    /* attend: a copy from the pools did not arrive in about 2 s: outputs are invalid */
 int kv_paged_error(KvPaged *kv);
@@ -134,11 +134,13 @@ int kv_paged_append(KvPaged *kv, const float *q, const float *k, const float *v,
  * out[r][h] = sum_t p_t v_t with p = softmax(scale * q[r][h] . k_t), in
  * float. row_pos -1 gives zeros; a row with row_request < 0 is passed over
  * and its output left as it was. Entries of the pools behind a row's
- * position are never used, whatever they hold; visible entries of an F32 pool
- * are below 2^127 in size. table has n_requests
- * (<= max_requests) rows. q and out: rows of n_heads * head_size floats on
- * 16 bytes, q_stride as in kv_paged_append; out must not overlap q. Results do
- * not depend on timing: the same inputs give the same bits.
+ * position are never used, whatever they hold. A q or a visible entry that is
+ * not finite (or 2^127 and more, in an F32 pool) makes the outputs that it
+ * enters not finite, without regard to the signs of infinities. n is at
+ * most 65535; table has n_requests (<= max_requests) rows. q and out: rows of
+ * n_heads * head_size floats on 16 bytes, q_stride as in kv_paged_append; out
+ * must not overlap q. Results do not depend on timing: the same inputs give
+ * the same bits.
  */
 int kv_paged_attend(KvPaged *kv, const float *q, const void *k_pool, const void *v_pool, const int *table,
                     int n_requests, const int *row_request, const int *row_pos, int n, float scale, float *out,

@@ -111,6 +111,43 @@ def test_map_many_rows_over_several_ctas(torch):
     kv.close()
 
 
+@pytest.mark.parametrize("n,most,max_rows,off", [(50, 9000, 260001, 0), (50, 9000, 260001, 1), (1500, 400, 400003, 0),
+                                                 (3, 100000, 299999, 3)])
+def test_map_hundreds_of_thousands_of_rows(torch, n, most, max_rows, off):
+    """More rows than threads: four of them a thread, stored in 16 bytes where
+    the lists lie on 16 bytes (off 0) and singly where they do not."""
+    page = 24
+    rng = np.random.default_rng(n)
+    blocks = -(-most // page)
+    n_pages = n * blocks
+    kv = pk_b200.KvPaged(1, 1, 8, pk_b200.F32, page, n_pages, n, blocks)
+    start = rng.integers(0, 3, n) * (rng.random(n) < 0.3)
+    end = np.maximum(start, np.minimum(rng.integers(0, most + 1, n), (max_rows - 5) // n))
+    length = start + rng.integers(0, 2, n)
+    length = np.minimum(length, most)
+    table = np.full((n, blocks), -1)
+    ids = rng.permutation(n_pages).tolist()
+    for i in range(n):
+        for b in range(ref.pages_of(int(length[i]), page)):
+            table[i, b] = ids.pop()
+    want = ref.map_step(length.tolist(), start.tolist(), end.tolist(), table.tolist(), ids, page, n_pages, max_rows)
+    assert want[0] == 0 and max_rows > 148 * 1024
+    d = [ints(torch, x) for x in (length, start, end)]
+    tb, stack, nf = ints(torch, table), ints(torch, ids + [-5] * (n_pages - len(ids))), ints(torch, [len(ids)])
+    rows = [torch.full((max_rows + 4,), -77, dtype=torch.int32, device="cuda") for _ in range(3)]
+    row0 = torch.empty(n + 1, dtype=torch.int32, device="cuda")
+    kv.map(d[0].data_ptr(), d[1].data_ptr(), d[2].data_ptr(), n, tb.data_ptr(), stack.data_ptr(), nf.data_ptr(),
+           nf.data_ptr(), max_rows, *(r.data_ptr() + 4 * off for r in rows), row0.data_ptr())
+    assert kv.error() == 0 and row0.cpu().tolist() == want[4] and tb.cpu().tolist() == want[1]
+    assert stack[:int(nf[0])].cpu().tolist() == want[2]
+    got = np.stack([r[off:off + max_rows].cpu().numpy() for r in rows], 1)
+    count = len(want[3])
+    assert np.array_equal(got[:count], np.asarray(want[3])) and (got[count:] == -1).all()
+    for r in rows:  # nothing around the lists was written
+        assert (r[:off] == -77).all() and (r[off + max_rows:] == -77).all()
+    kv.close()
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(start=[3, 6, 0]), ref.BAD_LENGTH), (dict(start=[-1, 5, 0]), ref.BAD_LENGTH), (dict(end=[2, 6, 1]), ref.BAD_LENGTH),
     (dict(end=[3, 17, 1]), ref.BAD_LENGTH), (dict(length=[3, 2 ** 31 - 1, 0]), ref.BAD_LENGTH),
@@ -361,8 +398,9 @@ def test_attend_against_64_bits(torch, kind, heads, kvh, hs, page):
 
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 @pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
-def test_attend_never_uses_what_is_behind_a_row(torch, kind, value):
-    s = Setup(torch, kind, "token", 8, 2, 64, 16, [1, 5, 16, 18, 47, 100, 0, 130])
+@pytest.mark.parametrize("hs,page", [(64, 16), (64, 7), (128, 8), (128, 64), (80, 24), (136, 32), (256, 5)])
+def test_attend_never_uses_what_is_behind_a_row(torch, kind, value, hs, page):
+    s = Setup(torch, kind, "token", 8, 2, hs, page, [1, 5, 16, 18, 47, 100, 0, 130])
     s.spoil(value)
     out = s.run()
     assert np.isfinite(out).all()
@@ -430,6 +468,52 @@ def test_attend_sizes_of_q(torch, kind, q_scale):
     assert np.isfinite(out).all()
     s.check(out)
     s.kv.close()
+
+
+@pytest.mark.parametrize("n,kind", [(127, "f32"), (129, "f16"), (1000, "f16"), (5000, "f32")])
+def test_attend_many_rows(torch, n, kind):
+    """More rows than a CTA has threads, some passed over, over few requests
+    and pages."""
+    rng = np.random.default_rng(n)
+    s = Setup(torch, kind, "head", 4, 2, 64, 8, [60, 33, 90, 0, 7])
+    s.req = rng.integers(-1, 5, n)
+    s.pos = np.array([rng.integers(-1, max(1, s.lens[i])) if i >= 0 else 3 for i in s.req])
+    s.pos[s.req == 3] = -1
+    s.q = rng.standard_normal((n, 4, 64)).astype(np.float32)
+    s.check(s.run())
+    assert s.kv.error() == 0
+    s.kv.close()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_attend_nan_stays_in_its_head(torch, kind):
+    """A query or a value that is not a number spoils its own heads only."""
+    s = Setup(torch, kind, "token", 8, 2, 64, 16, [300, 300, 40])
+    good = s.run()
+    s.q[0, 3, 5] = np.nan
+    s.v[s.table[1, 2], 4, 1, 7] = np.nan  # request 1, KV head 1: query heads 4 .. 7, channel 7
+    out = s.run()
+    bad = np.isnan(out)
+    assert bad[0, 3].all() and bad[1, 4:, 7].all() and bad.sum() == 64 + 4
+    assert np.array_equal(out[~bad], good[~bad])
+    s.kv.close()
+
+
+def test_attend_refuses_too_much_work(torch):
+    """2^31 chunks (a billion tokens for each of 256 KV heads) give an error
+    bit and no output; the table is one page again and again."""
+    page, blocks = 1 << 20, 1 << 10
+    kv = pk_b200.KvPaged(256, 256, 8, pk_b200.F16, page, 1, 1, blocks)
+    kp = torch.zeros(page * 256 * 8, device="cuda", dtype=torch.float16)
+    q, out = torch.zeros(1, 256, 8, device="cuda"), torch.full((1, 256, 8), -7.0, device="cuda")
+    tb, rr, rp = ints(torch, [[0] * blocks]), ints(torch, [0]), ints(torch, [(1 << 30) - 1])
+    args = (q.data_ptr(), kp.data_ptr(), kp.data_ptr(), tb.data_ptr(), 1, rr.data_ptr(), rp.data_ptr(), 1, 1.0, out.data_ptr())
+    kv.attend(*args)
+    assert kv.error() == 32 and (out == -7).all()
+    rp.fill_(1000)
+    kv.attend(*args)
+    assert kv.error() == 0 and (out == 0).all()
+    kv.close()
 
 
 def test_attend_bad_pages_and_rows(torch):
@@ -601,6 +685,33 @@ def test_steps_captured_once_and_replayed(torch, kind):
     g.replay()
     assert s.kv.error() == ref.NO_ROWS
     assert (s.out == -7).all()
+    s.kv.close()
+
+
+def test_two_graphs_of_one_handle_in_turn(torch):
+    """Two captured calls that share a handle's scratch, replayed one after
+    the other on one stream, with lengths that change between replays."""
+    s = Setup(torch, "f16", "token", 32, 8, 128, 16, [3000, 900, 1])
+    s.run()
+    st, graphs, outs = torch.cuda.Stream(), [], []
+    p = [x.data_ptr() for x in s.d]
+    for rows in (3, 2):
+        out = torch.full((3, 32, 128), -7.0, device="cuda")
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            s.kv.attend(p[0], p[1], p[2], p[3], 3, p[4], p[5], rows, s.scale, out.data_ptr(),
+                        stream=torch.cuda.current_stream().cuda_stream)
+        graphs.append(g)
+        outs.append(out)
+    for lens in ([3000, 900, 1], [1, 17, 0], [2049, 1, 1], [3000, 900, 1]):
+        s.pos = np.asarray(lens) - 1
+        s.d[5].copy_(ints(torch, s.pos))
+        for g in graphs:
+            g.replay()
+        a, b = (o.cpu().numpy() for o in outs)
+        s.check(a)
+        assert np.array_equal(a[:2], b[:2]) and (b[2] == -7).all()
+    assert s.kv.error() == 0
     s.kv.close()
 
 
