@@ -382,11 +382,12 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
 // one CTA's share are written at once; of the others each CTA leaves its
 // part in the scratch, and the last to arrive joins them, in their order.
 //
-// Where pages are whole multiples of 8 tokens, tensor maps over the pools
-// bring a tile in boxes of 128 bytes by 8 to 32 tokens (BOXES), a few
-// instructions a tile; else each lane copies 16 bytes at a time. Both lay a
-// box's 16-byte pieces out as the maps' 128-byte swizzle does (piece c of
-// token r at c ^ (r mod 8)), so that reads of eight tokens meet no bank twice.
+// Where pages are multiples of 8 tokens and heads of 128 bytes, tensor maps
+// over the pools bring a tile in boxes of 8 to 32 tokens (BOXES), two to
+// eight instructions a tile; else each lane copies 16 bytes at a time. Both
+// lay a column's 16-byte pieces out as the maps' 128-byte swizzle does (piece
+// c of token r at c ^ (r mod 8)), so that reads of eight tokens meet no bank
+// twice.
 // Tokens that a row may not see do not count: copies leave them out or, in
 // the box that a row ends in, their values are zeroed before use.
 constexpr int ATT_HEADS = 8;
@@ -405,9 +406,8 @@ struct Geo {
     static constexpr int STAGES = HSP == 256 || (HALF && HSP == 128) ? 1 : 2;
     static constexpr int CTAS = HSP == 256 ? 2 : 3;  // per SM, as shared memory allows
     static constexpr int CHUNK = WARPS * TILE;       // tokens: the unit in which work is shared out
-    static constexpr int WIDE = HSP * (int)sizeof(KV) / 128;  // boxes side by side
-    static constexpr int BOX = TILE * 128;                    // bytes of a column of boxes
-    static constexpr int SIDE = WIDE * BOX;                   // of a tile's keys; its values follow
+    static constexpr int WIDE = HSP * (int)sizeof(KV) / 128;  // columns of 128 bytes
+    static constexpr int SIDE = WIDE * TILE * 128;            // bytes of a tile's keys; its values follow
     static constexpr int STAGE = 2 * SIDE;
     static constexpr int RING = STAGES * STAGE;
     static constexpr int SEGS = HSP * (int)sizeof(KV) / 16;  // 16-byte pieces of a token's head
@@ -732,6 +732,18 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
         nx_head = l_head;
         l_tok += CHUNK;
     };
+    // A tile's side lies box after box, a box column after column of 128
+    // bytes, a column token after token; where the tile's tokens 8i .. 8i + 7
+    // begin (without BOXES: in one box).
+    const uint32_t column = BOXES ? 128u << unit_shift : TILE * 128;
+    auto eight = [&](int i) -> uint32_t {
+        if constexpr (BOXES) {
+            const int in_box = unit_shift - 3;
+            return (uint32_t)(i >> in_box) * G::WIDE * column + (uint32_t)(i & ((1 << in_box) - 1)) * 1024;
+        } else {
+            return i * 1024;
+        }
+    };
     const uint32_t bar_s = (uint32_t)__cvta_generic_to_shared(&bars[warp][0]);
     uint32_t phases = 0;   // of the warp's barriers, a bit a stage
     bool written = false;  // the slot that is filled next was written by this warp
@@ -764,16 +776,16 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                     asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
                 }
                 __syncwarp();
-                // a lane a box: of keys or values, of the boxes side by side, of the tile's tokens
-                const int sub = lane / (2 * G::WIDE), col = (lane >> 1) % G::WIDE;
+                // a lane a box, of keys or of values
+                const int sub = lane >> 1;
                 const int bp = __shfl_sync(0xFFFFFFFFu, page, sub), bl = __shfl_sync(0xFFFFFFFFu, place, sub);
                 if ((there >> sub) & 1u) {
-                    const uint32_t dst = dst0 + (lane & 1) * G::SIDE + col * G::BOX + (uint32_t)(sub * 128 << unit_shift);
+                    const uint32_t dst = dst0 + (lane & 1) * G::SIDE + (uint32_t)sub * G::WIDE * column;
                     const CUtensorMap *map = (lane & 1) ? &v_map : &k_map;
                     asm volatile(
-                        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-                        "%4, %5}], [%6];" ::"r"(dst),
-                        "l"(map), "r"(col * (128 / (int)sizeof(KV))), "r"(head), "r"(bl), "r"(bp), "r"(bar)
+                        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                        "%2, %4, %5}], [%6];" ::"r"(dst),
+                        "l"(map), "r"(0), "r"(bl), "r"(head), "r"(bp), "r"(bar)
                         : "memory");
                 }
             } else {
@@ -788,7 +800,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                     const bool in = ((there >> key) & 1u) && seg < segs;
                     const int bytes = in ? 16 : 0;
                     const uint64_t e = in ? (uint64_t)(from + seg) * 16 : 0;
-                    const uint32_t dst = dst0 + (seg >> 3) * G::BOX + key * 128 + (((seg ^ key) & 7) << 4);
+                    const uint32_t dst = dst0 + (seg >> 3) * column + key * 128 + (((seg ^ key) & 7) << 4);
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst),
                                  "l"(static_cast<const uint8_t *>(a.k_pool) + e), "r"(bytes)
                                  : "memory");
@@ -876,6 +888,14 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
         qa[3] = v.w;
     };
 
+    // where the eight tokens of a lane's addresses begin: of 16 keys (half) or 8
+    uint32_t k_eight[G::HALF ? NT / 2 : NT], v_eight[G::HALF ? NT / 2 : NT];
+#pragma unroll
+    for (int j = 0; j < (G::HALF ? NT / 2 : NT); j++) {
+        k_eight[j] = eight(G::HALF ? 2 * j + (lane >> 4) : j);
+        v_eight[j] = eight(G::HALF ? 2 * j + ((lane >> 3) & 1) : j);
+    }
+
     // ---- items of the share: one loop, so that each part of it is there once
     // (instructions that a warp meets for the first time cost it a fetch) ----
     ask_q(cp);  // ahead of the tiles: behind them it would wait for what all CTAs ask for
@@ -933,9 +953,12 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
             if (BOXES && mask != (uint32_t)((1ull << TILE) - 1)) {
                 // tokens that do not count: what they hold must not meet p = 0
                 for (int i = lane; i < TILE * 8 * G::WIDE; i += 32) {
-                    const int key = (i >> 3) % TILE;
+                    const int key = i % TILE, seg = i / TILE;
                     if (!((mask >> key) & 1u))
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs_s + 16 * i), "r"(0u) : "memory");
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(
+                                         vs_s + eight(key >> 3) + (key & 7) * 128 + (seg >> 3) * column + (seg & 7) * 16),
+                                     "r"(0u)
+                                     : "memory");
                 }
                 written = true;
                 __syncwarp();
@@ -945,7 +968,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
 #pragma unroll
                 for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
                 if constexpr (G::HALF) {
-                    const uint32_t at = ks_s + ((lane >> 4) * 8 + (lane & 7)) * 128, piece = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
+                    const uint32_t at = ks_s + (lane & 7) * 128, piece = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
 #pragma unroll
                     for (int ks = 0; ks < KS; ks++) {
                         uint32_t qa[4];
@@ -953,7 +976,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
 #pragma unroll
                         for (int j = 0; j < NT / 2; j++) {
                             uint32_t kb[4];
-                            ldmatrix4(kb, at + (ks / 4) * G::BOX + 16 * j * 128 + (piece ^ ((ks & 3) << 5)));
+                            ldmatrix4(kb, at + k_eight[j] + (ks / 4) * column + (piece ^ ((ks & 3) << 5)));
                             mma_f16(s[2 * j], qa, kb[0], kb[1]);
                             mma_f16(s[2 * j + 1], qa, kb[2], kb[3]);
                         }
@@ -971,7 +994,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
 #pragma unroll
                         for (int j = 0; j < NT; j++) {
                             uint32_t kb[4];
-                            ldmatrix4(kb, at + (ks / 2) * G::BOX + 8 * j * 128 + (piece ^ ((ks & 1) << 6)));
+                            ldmatrix4(kb, at + k_eight[j] + (ks / 2) * column + (piece ^ ((ks & 1) << 6)));
                             mma_tf32(s[j], qa, kb[0], kb[1]);
                             mma_tf32(s2[j], qa, rest_tf32(kb[0]), rest_tf32(kb[1]));
                             mma_tf32(s[j], qb, kb[2], kb[3]);
@@ -1017,7 +1040,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                         split_f16(p[2 * kb][0], p[2 * kb][1], pa[kb][0], pa[kb][1]);
                         split_f16(p[2 * kb + 1][0], p[2 * kb + 1][1], pa[kb][2], pa[kb][3]);
                     }
-                    const uint32_t at = vs_s + (((lane >> 3) & 1) * 8 + (lane & 7)) * 128;
+                    const uint32_t at = vs_s + (lane & 7) * 128;
                     const uint32_t piece = ((lane >> 4) ^ (lane & 7)) << 4;
 #pragma unroll
                     for (int i = 0; i < DT / 2; i++) {
@@ -1025,7 +1048,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
 #pragma unroll
                         for (int kb = 0; kb < TILE / 16; kb++) {
                             uint32_t vb[4];
-                            ldmatrix4_t(vb, at + (i / 4) * G::BOX + 16 * kb * 128 + (piece ^ ((i & 3) << 5)));
+                            ldmatrix4_t(vb, at + v_eight[kb] + (i / 4) * column + (piece ^ ((i & 3) << 5)));
                             mma_f16(x, pa[kb], vb[0], vb[1]);
                             mma_f16(y, pa[kb], vb[2], vb[3]);
                         }
@@ -1047,7 +1070,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                         float s4[4][4];
 #pragma unroll
                         for (int kb = 0; kb < NT; kb++) {
-                            const uint8_t *vk = v0 + c * G::BOX + 8 * kb * 128;
+                            const uint8_t *vk = v0 + v_eight[kb] + c * column;
                             const float4 x = *reinterpret_cast<const float4 *>(vk + ((g ^ (2 * t4)) << 4));
                             const float4 y = *reinterpret_cast<const float4 *>(vk + 128 + ((g ^ (2 * t4 + 1)) << 4));
                             const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
@@ -1348,20 +1371,22 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_tiled()
     return fn;
 }
 
-// The map of a pool: channels, KV heads, a page's tokens, pages; boxes of 128
-// bytes by 2^box_shift tokens. Channels past the head size read as 0.
+// The map of a pool: a column's 128 bytes of channels, a page's tokens, the
+// columns of a head, KV heads, pages; a box is all columns of 2^box_shift
+// tokens. Columns past the head size read as 0.
 static bool pool_map(const KvPaged *kv, const void *pool, CUtensorMap *map)
 {
     const KvPagedShape &s = kv->s;
-    const cuuint64_t size = s.type == 1 ? 2 : 4;
-    const cuuint64_t dims[4] = {(cuuint64_t)s.head_size, (cuuint64_t)s.n_kv_heads, (cuuint64_t)s.page_tokens,
+    const cuuint64_t size = s.type == 1 ? 2 : 4, wide = 128 / size;
+    const cuuint64_t dims[5] = {wide, (cuuint64_t)s.page_tokens, s.head_size / wide, (cuuint64_t)s.n_kv_heads,
                                 (cuuint64_t)s.n_pages};
     // the stride of an axis with a single entry is never used, but must be a proper one
-    auto stride = [&](uint64_t entries, int count) { return count > 1 ? entries * size : (cuuint64_t)16; };
-    const cuuint64_t strides[3] = {stride(s.head_stride, s.n_kv_heads), stride(s.token_stride, s.page_tokens),
+    auto stride = [&](uint64_t entries, int count) { return count > 1 ? entries * size : (cuuint64_t)128; };
+    const cuuint64_t strides[4] = {stride(s.token_stride, s.page_tokens), 128, stride(s.head_stride, s.n_kv_heads),
                                    stride(s.page_stride, s.n_pages)};
-    const cuuint32_t box[4] = {(cuuint32_t)(128 / size), 1, 1u << kv->box_shift, 1}, step[4] = {1, 1, 1, 1};
-    return encode_tiled()(map, s.type == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
+    const cuuint32_t box[5] = {(cuuint32_t)wide, 1u << kv->box_shift, (cuuint32_t)(kv->hsp / wide), 1, 1};
+    const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+    return encode_tiled()(map, s.type == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 5,
                           const_cast<void *>(pool), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1378,7 +1403,7 @@ static auto with_attend(const KvPaged *kv, F use)
         Geo<KV, HSP, BOXES>::TILE)
 #define KVP_CASE(KV, HSP) (kv->boxes ? KVP_KERNEL(KV, HSP, true) : KVP_KERNEL(KV, HSP, false))
     if (kv->s.type == 1) return kv->hsp == 64 ? KVP_CASE(__half, 64) : kv->hsp == 128 ? KVP_CASE(__half, 128) : KVP_CASE(__half, 256);
-    return kv->hsp == 64 ? KVP_CASE(float, 64) : kv->hsp == 128 ? KVP_CASE(float, 128) : KVP_KERNEL(float, 256, false);
+    return kv->hsp == 64 ? KVP_CASE(float, 64) : kv->hsp == 128 ? KVP_CASE(float, 128) : KVP_CASE(float, 256);
 #undef KVP_KERNEL
 #undef KVP_CASE
 }
@@ -1421,8 +1446,7 @@ extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *e
         OnDevice on(device);
         e = on.ok ? cudaDeviceGetAttribute(&kv->sms, cudaDevAttrMultiProcessorCount, device) : cudaErrorInvalidDevice;
         size_t parts = 0;
-        // 256 floats are 16 boxes of 1 KB a tile: 122 us for 32 rows of 2000 tokens, 102 us by 16-byte copies
-        kv->boxes = s.page_tokens % 8 == 0 && !(s.type == 0 && s.head_size > 128) && encode_tiled() != nullptr;
+        kv->boxes = s.page_tokens % 8 == 0 && s.head_size * (s.type == 1 ? 2 : 4) % 128 == 0 && encode_tiled() != nullptr;
         kv->hsp = s.head_size <= 64 ? 64 : s.head_size <= 128 ? 128 : 256;
         if (e == cudaSuccess) {
             e = with_attend(kv, [&](auto kernel, int threads, int smem, int floats, int tile) {
