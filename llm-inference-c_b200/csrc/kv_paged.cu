@@ -424,7 +424,7 @@ struct AttendArgs {
     const int *table, *row_request, *row_pos;
     int n, n_requests, heads, kv_heads, hs;
     int groups, group_heads;  // a KV head's items, and the query heads of each
-    Div by_groups, by_f4;     // f4: head size / 4
+    Div by_groups, by_f4, by_grid;  // f4: head size / 4
     float scale;
     float *out;
     uint64_t q_stride;
@@ -624,11 +624,15 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
     const int each = (a.n + 32 * W - 1) / (32 * W), r0 = min(a.n, tid * each), r1 = min(a.n, r0 + each);
     int fault = 0;
     long long mine = 0;
-    int longest = 0;
+    int longest = 0, req0 = -1, tokens0 = -1;  // of this thread's rows; its first row
     for (int r = r0; r < r1; r++) {
         const int req = a.row_request[r], tokens = row_tokens(a, req, a.row_pos[r], fault), u = units_of<CHUNK>(tokens);
         mine += (long long)u * items;
         longest = max(longest, u);
+        if (r == r0) {
+            req0 = req;
+            tokens0 = tokens;
+        }
     }
     if (fault && b == 0) atomicOr(a.err, fault);
     // sums in 32 bits, and those of 256ths, which cannot overflow, beside them
@@ -654,7 +658,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
         much += x.y;
         longest = max(longest, (int)x.z);
     }
-    if (much >= (1u << 23) - 32 * W) {
+    if (much >= (1u << 23) - 32 * W - 64) {
         if (b == 0 && tid == 0) atomicOr(a.err, KV_PAGED_TOO_MUCH);
         return;
     }
@@ -662,14 +666,15 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
     // is not full about 1 us: where that leaves less to all CTAs, shares are
     // not smaller than makes both sides equal for the longest item, whose
     // parts are longest / share, nor than a chunk and an item's end.
-    const unsigned even = (all + gridDim.x - 1) / gridDim.x;
+    const unsigned even = (unsigned)div_by(a.by_grid, (int)(all + gridDim.x - 1));
     const unsigned share = max(max(even, 2u), (unsigned)__fsqrt_rn(ATT_JOIN * longest));
     const unsigned first = (unsigned)min((unsigned long long)share * b, 1ull << 31);
     if (first >= all) return;
     if (first - before < own) {
         unsigned at = before;
         for (int r = r0; r < r1; r++) {
-            const int req = a.row_request[r], tokens = row_tokens(a, req, a.row_pos[r], fault);
+            const int req = r == r0 ? req0 : a.row_request[r];
+            const int tokens = r == r0 ? tokens0 : row_tokens(a, req, a.row_pos[r], fault);
             const unsigned u = units_of<CHUNK>(tokens);
             if (first - at < u * items) {
                 begin.r = r;
@@ -1634,6 +1639,7 @@ extern "C" int kv_paged_attend(KvPaged *kv, const float *q, const void *k_pool, 
     a.group_heads = (group + a.groups - 1) / a.groups;
     a.by_groups = kvp::make_div((uint32_t)a.groups);
     a.by_f4 = kvp::make_div((uint32_t)s.head_size / 4);
+    a.by_grid = kvp::make_div((uint32_t)kv->grid);
     a.scale = scale;
     a.out = out;
     a.q_stride = q_stride;
