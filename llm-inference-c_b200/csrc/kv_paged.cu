@@ -97,9 +97,12 @@ __host__ __device__ __forceinline__ int pages_of(const Div &page, int x)
 // read it.
 //
 // A step of few rows is one CTA and bound by its chain of three loads from
-// memory (lengths, pages, then the rows' stores); many rows are bound by
-// their 12 bytes each: a thread then finds the request of ROWS = 4 rows with
-// one search and stores them in 16 bytes.
+// memory (lengths, pages, then the rows' stores): 64 requests take 3.0 us. Many
+// rows are bound by their 12 bytes each: a thread then finds the request of
+// ROWS = 4 rows with one search and stores them in 16 bytes (two million rows
+// of 256 requests 10 us, 2.5 TB/s; a row a thread 17 us). More than 1024
+// requests take CTAs of 1024 threads, since every CTA sums over all of them
+// (4096 requests 13 us, with 256 threads 27).
 template <int THREADS, int ROWS>
 __global__ void __launch_bounds__(THREADS) map_kernel(const MapArgs a)
 {
@@ -287,7 +290,7 @@ struct AppendArgs {
     int *err;
 };
 
-constexpr int APP_THREADS = 256, APP_AHEAD = 4;
+constexpr int APP_THREADS = 128, APP_AHEAD = 4;
 
 // Four entries, rounded as the cache holds them.
 __device__ __forceinline__ void kv_store4(float *p, float4 v)
@@ -302,9 +305,11 @@ __device__ __forceinline__ void kv_store4(__half *p, float4 v)
 }
 
 // CTA (r, y) takes every gridDim.y-th stretch of row r's q, k and v, in 16
-// bytes a thread, APP_AHEAD loads in flight: a copy, bound by memory. A
-// pair's two products and their sum are each rounded, as the decode step
-// does.
+// bytes a thread, APP_AHEAD loads in flight: a copy, bound by memory. 16384
+// rows of 32 heads and 8 KV heads of 128 into a half cache, 747 MB, take
+// 115 us, 6.5 TB/s, what a copy reaches; with 256 threads 134 us (fewer CTAs
+// to fill an SM with), with loads marked as read once 121. A pair's two
+// products and their sum are each rounded, as the decode step does.
 template <typename KV>
 __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
 {
@@ -319,7 +324,9 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
 #pragma unroll
         for (int j = 0; j < APP_AHEAD; j++) {
             const int i = i0 + j * step;
-            if (i < all) x[j] = __ldcs(reinterpret_cast<const float4 *>(i < q4 ? q + 4 * i : i < q4 + k4 ? k + 4 * (i - q4) : v + 4 * (i - q4 - k4)));
+            if (i >= all) break;
+            const float *from = i < q4 ? q + 4 * i : i < q4 + k4 ? k + 4 * (i - q4) : v + 4 * (i - q4 - k4);
+            x[j] = *reinterpret_cast<const float4 *>(from);
         }
         if (i0 < APP_AHEAD * step) {
             if (slot < 0) return;
@@ -390,6 +397,12 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
 // twice.
 // Tokens that a row may not see do not count: copies leave them out or, in
 // the box that a row ends in, their values are zeroed before use.
+//
+// Bound by the pools' bytes: 64 rows of up to 8192 tokens (half, 32 heads, 8
+// KV heads of 128; 1.16 GB) take 181 us, 6.4 TB/s, as a copy reaches; 16 rows
+// of 1030 (float, 32 KV heads; 540 MB) 90 us, 6.0 TB/s. Few tokens are bound by
+// the chain of a row's numbers, a page's, a tile and the products: one row of
+// 40 takes 5 us, one of 2000 11 us, of which joining its parts is 4.
 constexpr int ATT_HEADS = 8;
 constexpr float ATT_JOIN = 0.2f;  // the cost of a part over that of a chunk
 
