@@ -504,8 +504,8 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
 }
-// o = o f + the sum of both halves of a tile's product. The running sums are
-// kept outside the tensor cores, whose accumulators cut bits off instead of
+// o = o f + the sum of both halves of a product. The running sums are kept
+// outside the tensor cores, whose accumulators cut bits off instead of
 // rounding: over a thousand tokens that adds up to 2e-6 of the result, always
 // towards zero.
 __device__ __forceinline__ void add_tile(float (&o)[2], const float (&x)[4], float f)
@@ -982,27 +982,38 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                 __syncwarp();
             }
             if (mask != 0u) {
-                float s[NT][4];
+                // Scores are added up like values: a few products in the tensor
+                // cores, the rest outside (a chain of all 128 channels there
+                // takes 1e-6 off the result, of 1030 tokens, always to one side).
+                float s[NT][2];
 #pragma unroll
-                for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+                for (int j = 0; j < NT; j++) s[j][0] = s[j][1] = 0.0f;
                 if constexpr (G::HALF) {
                     const uint32_t at = ks_s + (lane & 7) * 128, piece = (((lane >> 3) & 1) ^ (lane & 7)) << 4;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ks++) {
-                        uint32_t qa[4];
-                        q_step(ks, qa);
+                    for (int k2 = 0; k2 < KS / 2; k2++) {
+                        float z[NT][4];
 #pragma unroll
-                        for (int j = 0; j < NT / 2; j++) {
-                            uint32_t kb[4];
-                            ldmatrix4(kb, at + k_eight[j] + (ks / 4) * column + (piece ^ ((ks & 3) << 5)));
-                            mma_f16(s[2 * j], qa, kb[0], kb[1]);
-                            mma_f16(s[2 * j + 1], qa, kb[2], kb[3]);
+                        for (int j = 0; j < NT; j++) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.0f;
+#pragma unroll
+                        for (int ks = 2 * k2; ks < 2 * k2 + 2; ks++) {
+                            uint32_t qa[4];
+                            q_step(ks, qa);
+#pragma unroll
+                            for (int j = 0; j < NT / 2; j++) {
+                                uint32_t kb[4];
+                                ldmatrix4(kb, at + k_eight[j] + (ks / 4) * column + (piece ^ ((ks & 3) << 5)));
+                                mma_f16(z[2 * j], qa, kb[0], kb[1]);
+                                mma_f16(z[2 * j + 1], qa, kb[2], kb[3]);
+                            }
                         }
+#pragma unroll
+                        for (int j = 0; j < NT; j++) add_tile(s[j], z[j], 1.0f);
                     }
                 } else {
-                    float s2[NT][4];  // the lower parts' products, a second chain
+                    float rest[NT][4];  // the lower parts' products, small enough to stay in one chain
 #pragma unroll
-                    for (int j = 0; j < NT; j++) s2[j][0] = s2[j][1] = s2[j][2] = s2[j][3] = 0.0f;
+                    for (int j = 0; j < NT; j++) rest[j][0] = rest[j][1] = rest[j][2] = rest[j][3] = 0.0f;
                     const uint32_t at = ks_s + (lane & 7) * 128, piece = ((lane >> 3) ^ (lane & 7)) << 4;
 #pragma unroll
                     for (int ks = 0; ks < KS / 2; ks++) {
@@ -1013,16 +1024,16 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                         for (int j = 0; j < NT; j++) {
                             uint32_t kb[4];
                             ldmatrix4(kb, at + k_eight[j] + (ks / 2) * column + (piece ^ ((ks & 1) << 6)));
-                            mma_tf32(s[j], qa, kb[0], kb[1]);
-                            mma_tf32(s2[j], qa, rest_tf32(kb[0]), rest_tf32(kb[1]));
-                            mma_tf32(s[j], qb, kb[2], kb[3]);
-                            mma_tf32(s2[j], qb, rest_tf32(kb[2]), rest_tf32(kb[3]));
+                            float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_tf32(z, qa, kb[0], kb[1]);
+                            mma_tf32(rest[j], qa, rest_tf32(kb[0]), rest_tf32(kb[1]));
+                            mma_tf32(z, qb, kb[2], kb[3]);
+                            mma_tf32(rest[j], qb, rest_tf32(kb[2]), rest_tf32(kb[3]));
+                            add_tile(s[j], z, 1.0f);
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < NT; j++)
-#pragma unroll
-                        for (int i = 0; i < 4; i++) s[j][i] += s2[j][i];
+                    for (int j = 0; j < NT; j++) add_tile(s[j], rest[j], 1.0f);
                 }
                 // head g's scores of tokens 8j + 2 t4 and the next one
                 float top = -INFINITY, p[NT][2];
@@ -1030,7 +1041,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                 for (int j = 0; j < NT; j++) {
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
-                        p[j][i] = (s[j][i] + s[j][i + 2]) * unit;
+                        p[j][i] = s[j][i] * unit;
                         if (!((mask >> (8 * j + 2 * t4 + i)) & 1u)) p[j][i] = -INFINITY;
                         top = fmaxf(top, p[j][i]);
                     }
