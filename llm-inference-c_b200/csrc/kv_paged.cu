@@ -233,10 +233,13 @@ __global__ void __launch_bounds__(THREADS) map_kernel(const MapArgs a)
             pos[k] = p;
             if (page >= 0 && page < a.c.n_pages) slot[k] = page * (int)a.c.page.d + (p - blk * (int)a.c.page.d);
         }
-        if (ROWS == 4 && wide && r0 + ROWS <= a.max_rows) {
-            *reinterpret_cast<int4 *>(a.row_request + r0) = make_int4(req[0], req[1 % ROWS], req[2 % ROWS], req[3 % ROWS]);
-            *reinterpret_cast<int4 *>(a.row_pos + r0) = make_int4(pos[0], pos[1 % ROWS], pos[2 % ROWS], pos[3 % ROWS]);
-            *reinterpret_cast<int4 *>(a.row_slot + r0) = make_int4(slot[0], slot[1 % ROWS], slot[2 % ROWS], slot[3 % ROWS]);
+        if (ROWS > 1 && wide && r0 + ROWS <= a.max_rows) {
+#pragma unroll
+            for (int k = 0; k + 3 < ROWS; k += 4) {
+                *reinterpret_cast<int4 *>(a.row_request + r0 + k) = make_int4(req[k], req[k + 1], req[k + 2], req[k + 3]);
+                *reinterpret_cast<int4 *>(a.row_pos + r0 + k) = make_int4(pos[k], pos[k + 1], pos[k + 2], pos[k + 3]);
+                *reinterpret_cast<int4 *>(a.row_slot + r0 + k) = make_int4(slot[k], slot[k + 1], slot[k + 2], slot[k + 3]);
+            }
         } else {
 #pragma unroll
             for (int k = 0; k < ROWS; k++) {
