@@ -409,7 +409,7 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
 constexpr int ATT_HEADS = 8;
 constexpr float ATT_JOIN = 0.2f;  // the cost of a part over that of a chunk
 
-template <typename KV, int HSP, bool BOXES>
+template <typename KV, int HSP, bool BOXES, int PLAIN>
 struct Geo {
     static constexpr bool HALF = sizeof(KV) == 2;
     static constexpr int TILE = HALF ? (HSP <= 128 ? 32 : 16) : (HSP == 64 ? 16 : 8);  // tokens
@@ -428,7 +428,8 @@ struct Geo {
     static constexpr int RING = STAGES * STAGE;
     static constexpr int SEGS = HSP * (int)sizeof(KV) / 16;  // 16-byte pieces of a token's head
     static constexpr int KS = HALF ? HSP / 16 : HSP / 8;     // steps of a score's product
-    static constexpr int SMEM = 1024 + WARPS * RING + KS * 512;  // rings on 1024 bytes, then q as the left operand
+    static constexpr int QBYTES = PLAIN ? PLAIN * HSP * 4 : KS * 512;  // q, or q as the left operand
+    static constexpr int SMEM = 1024 + WARPS * RING + QBYTES;           // rings on 1024 bytes, then q
     static constexpr int OROW = HSP + 8;                     // floats from a head to the next of sums that wait to be joined
     static constexpr int PART = ATT_HEADS * OROW;            // floats of a part
     static_assert(PART * 4 <= STAGE, "a warp's sums fit a stage");
@@ -506,6 +507,25 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t &hi, uint32
     const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+// Two floats in 64 bits, and a b + c of both.
+__device__ __forceinline__ uint64_t pack2(float x, float y)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 // o = o f + the sum of both halves of a product. The running sums are kept
 // outside the tensor cores, whose accumulators cut bits off instead of
@@ -606,11 +626,11 @@ struct Part {
     int r, h0, heads, b0, parts;  // the item's first CTA, and how many hold it (0: no such part)
 };
 
-template <typename KV, int HSP, bool BOXES>
-__global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, BOXES>::CTAS)
+template <typename KV, int HSP, bool BOXES, int PLAIN>
+__global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES, PLAIN>::WARPS, Geo<KV, HSP, BOXES, PLAIN>::CTAS)
     attend_kernel(const AttendArgs a, const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map)
 {
-    using G = Geo<KV, HSP, BOXES>;
+    using G = Geo<KV, HSP, BOXES, PLAIN>;
     constexpr int TILE = G::TILE, CHUNK = G::CHUNK, W = G::WARPS, NT = TILE / 8, DT = HSP / 8, KS = G::KS;
     constexpr int JT = (ATT_HEADS * HSP / 4 + 32 * W - 1) / (32 * W);  // pieces of 4 channels of all heads, per thread
     constexpr int HW = (ATT_HEADS + W - 1) / W;  // heads of a warp
@@ -882,7 +902,10 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
 #pragma unroll
             for (int i = 0; i < HSP / 64; i++) {
                 const int d = 2 * lane + 64 * i;
-                if constexpr (G::HALF) {
+                if constexpr (PLAIN > 0) {
+                    if (h < PLAIN)
+                        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(qf) + h * HSP + d) = make_float2(x[2 * i], x[2 * i + 1]);
+                } else if constexpr (G::HALF) {
                     uint32_t hi, lo;
                     split_f16(x[2 * i], x[2 * i + 1], hi, lo);
                     const int kk = d & 15;
@@ -917,6 +940,16 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
         v_eight[j] = eight(G::HALF ? 2 * j + ((lane >> 3) & 1) : j);
     }
 
+    // PLAIN: lane (g, t4) multiplies key `plain_key` of eight (keys 4 apart in a
+    // quarter-warp, whose pieces the swizzle keeps apart) by pieces t4 and
+    // t4 + 4 of each column, and adds up values in piece `lane` of all, or
+    // (64 channels) piece lane mod 16 of every second token.
+    constexpr int PH = PLAIN ? PLAIN : 1, QP = PLAIN ? HSP / 16 : 1;    // pieces of q
+    constexpr int OP = PLAIN ? (HSP < 128 ? 1 : HSP / 128) : 1;          // pieces of o
+    const int plain_key = (g >> 1) | ((g & 1) << 2);
+    ulonglong2 qv[PH][QP], ov[PH][OP];
+    float pm[PH], pl[PH];
+
     // ---- items of the share: one loop, so that each part of it is there once
     // (instructions that a warp meets for the first time cost it a fetch) ----
     ask_q(cp);  // ahead of the tiles: behind them it would wait for what all CTAs ask for
@@ -928,8 +961,20 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
     bool lost = false;  // a tile did not arrive
     bool fresh = true, used = false;  // q is to be made; this warp has had a tile of the item
     float o[DT][2], m = -INFINITY, l = 0.0f, unit = 1.0f;
+    auto clear = [&]() {
+        m = -INFINITY;
+        l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
+        for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
+#pragma unroll
+        for (int h = 0; h < PH; h++) {
+            pm[h] = -INFINITY;
+            pl[h] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < OP; i++) ov[h][i] = make_ulonglong2(0ull, 0ull);
+        }
+    };
+    clear();
     if (tid < 2) pend[tid].parts = 0;
     Place<CHUNK> np = cp;
     while (true) {
@@ -944,6 +989,13 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
             if (cp.left == begin.left) make_q();
             __syncthreads();  // q is there, and the sums of the item before are read
             unit = head_unit[g];
+            if constexpr (PLAIN > 0) {
+#pragma unroll
+                for (int h = 0; h < PH; h++)
+#pragma unroll
+                    for (int i = 0; i < QP; i++)
+                        qv[h][i] = *reinterpret_cast<const ulonglong2 *>(reinterpret_cast<const float *>(qf) + h * HSP + 16 * i + 4 * t4);
+            }
             np.next(a, items);
             if (np.left > 0) ask_q(np);
             fresh = false;
@@ -984,7 +1036,82 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
                 written = true;
                 __syncwarp();
             }
-            if (mask != 0u) {
+            if (PLAIN > 0 && mask != 0u) {
+                const uint8_t *keys = ring + slot * G::STAGE, *values = keys + G::SIDE;
+                float s[PH][NT];
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const uint8_t *key = keys + eight(j) + plain_key * 128;
+                    uint64_t z[PH][2];
+#pragma unroll
+                    for (int h = 0; h < PH; h++) z[h][0] = z[h][1] = 0ull;
+#pragma unroll
+                    for (int i = 0; i < QP; i++) {
+                        const ulonglong2 k = *reinterpret_cast<const ulonglong2 *>(
+                            key + (i >> 1) * column + (((t4 + 4 * (i & 1)) ^ plain_key) << 4));
+#pragma unroll
+                        for (int h = 0; h < PH; h++) {
+                            z[h][0] = fma2(qv[h][i].x, k.x, z[h][0]);
+                            z[h][1] = fma2(qv[h][i].y, k.y, z[h][1]);
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < PH; h++) {
+                        const float2 a2 = unpack2(z[h][0]), b2 = unpack2(z[h][1]);
+                        float x = (a2.x + b2.x) + (a2.y + b2.y);
+                        x += __shfl_xor_sync(0xFFFFFFFFu, x, 1);
+                        x += __shfl_xor_sync(0xFFFFFFFFu, x, 2);
+                        s[h][j] = ((mask >> (8 * j + plain_key)) & 1u) ? x : -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < PH; h++) {
+                    float top = s[h][0];
+#pragma unroll
+                    for (int j = 1; j < NT; j++) top = fmaxf(top, s[h][j]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                    const float mn = fmaxf(pm[h], top), f = weight_of(pm[h], mn), base = mn == -INFINITY ? 0.0f : mn;
+                    pm[h] = mn;
+                    pl[h] *= f;
+                    const uint64_t f2 = pack2(f, f);
+#pragma unroll
+                    for (int i = 0; i < OP; i++) {
+                        ov[h][i].x = fma2(ov[h][i].x, f2, 0ull);
+                        ov[h][i].y = fma2(ov[h][i].y, f2, 0ull);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {
+                        s[h][j] = exp2_fast(s[h][j] - base);
+                        pl[h] += s[h][j];
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < TILE; r += HSP < 128 ? 2 : 1) {
+                    // the token of this lane's half, and the lane that has its p
+                    const int q = HSP < 128 ? r + (lane >> 4) : r, r8 = q & 7;
+                    const int from = 4 * (((r8 & 3) << 1) | (r8 >> 2));
+                    const uint8_t *row = values + eight(r >> 3) + r8 * 128;
+                    uint64_t p2[PH];
+#pragma unroll
+                    for (int h = 0; h < PH; h++) {
+                        const float p = __shfl_sync(0xFFFFFFFFu, s[h][r >> 3], from);
+                        p2[h] = pack2(p, p);
+                    }
+#pragma unroll
+                    for (int i = 0; i < OP; i++) {
+                        const int piece = HSP < 128 ? lane & 15 : lane + 32 * i;
+                        const ulonglong2 v =
+                            *reinterpret_cast<const ulonglong2 *>(row + (piece >> 3) * column + (((piece & 7) ^ r8) << 4));
+#pragma unroll
+                        for (int h = 0; h < PH; h++) {
+                            ov[h][i].x = fma2(p2[h], v.x, ov[h][i].x);
+                            ov[h][i].y = fma2(p2[h], v.y, ov[h][i].y);
+                        }
+                    }
+                }
+            }
+            if (PLAIN == 0 && mask != 0u) {
                 // Scores are added up like values: a few products in the tensor
                 // cores, the rest outside (a chain of all 128 channels there
                 // takes 1e-6 off the result, of 1030 tokens, always to one side).
@@ -1129,27 +1256,51 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
             hold = written = true;  // the last tile's slot is filled again after the item's end
         }
         // ---- the item's end: the warps' sums, each in the slot of its last tile ----
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
         float *mine_o = reinterpret_cast<float *>(ring + slot * G::STAGE);
-        if (used) {
-            float *dst = mine_o + g * G::OROW;
+        if constexpr (PLAIN > 0) {
 #pragma unroll
-            for (int i = 0; i < DT; i += G::HALF ? 1 : 4) {
-                if constexpr (G::HALF) {
-                    *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t4) = make_float2(o[i][0], o[i][1]);
-                } else {
+            for (int h = 0; h < PH; h++) {
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        *reinterpret_cast<float4 *>(dst + 8 * i + 8 * t4 + 4 * j) =
-                            make_float4(o[i][j], o[i + (G::HALF ? 0 : 1)][j], o[i + (G::HALF ? 0 : 2)][j],
-                                        o[i + (G::HALF ? 0 : 3)][j]);
+                for (int x = 4; x < 32; x <<= 1) pl[h] += __shfl_xor_sync(0xFFFFFFFFu, pl[h], x);
+#pragma unroll
+                for (int i = 0; i < OP; i++) {
+                    const float2 a2 = unpack2(ov[h][i].x), b2 = unpack2(ov[h][i].y);
+                    float4 x = make_float4(a2.x, a2.y, b2.x, b2.y);
+                    if (HSP < 128) {
+                        x.x += __shfl_xor_sync(0xFFFFFFFFu, x.x, 16);
+                        x.y += __shfl_xor_sync(0xFFFFFFFFu, x.y, 16);
+                        x.z += __shfl_xor_sync(0xFFFFFFFFu, x.z, 16);
+                        x.w += __shfl_xor_sync(0xFFFFFFFFu, x.w, 16);
+                    }
+                    const int piece = HSP < 128 ? lane & 15 : lane + 32 * i;
+                    if (used && (HSP >= 128 || lane < 16)) *reinterpret_cast<float4 *>(mine_o + h * G::OROW + 4 * piece) = x;
+                }
+                if (lane == 0) {
+                    wm[h][warp] = pm[h];
+                    wl[h][warp] = used ? pl[h] : 0.0f;
                 }
             }
-        }
-        if (t4 == 0) {
-            wm[g][warp] = m;
-            wl[g][warp] = used ? l : 0.0f;
+        } else {
+            l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+            l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+            if (used) {
+                float *dst = mine_o + g * G::OROW;
+#pragma unroll
+                for (int i = 0; i < DT; i += G::HALF ? 1 : 4) {
+                    if constexpr (G::HALF) {
+                        *reinterpret_cast<float2 *>(dst + 8 * i + 2 * t4) = make_float2(o[i][0], o[i][1]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; j++)
+                            *reinterpret_cast<float4 *>(dst + 8 * i + 8 * t4 + 4 * j) =
+                                make_float4(o[i][j], o[i + 1][j], o[i + 2][j], o[i + 3][j]);
+                    }
+                }
+            }
+            if (t4 == 0) {
+                wm[g][warp] = m;
+                wl[g][warp] = used ? l : 0.0f;
+            }
         }
         if (lane == 0) wo[warp] = mine_o;
         __syncthreads();
@@ -1201,10 +1352,7 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, 
         stop = cp.stop();
         fresh = true;
         used = false;
-        m = -INFINITY;
-        l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DT; i++) o[i][0] = o[i][1] = 0.0f;
+        clear();
     }
     if (!BOXES) asm volatile("cp.async.wait_all;" ::: "memory");
 
@@ -1430,14 +1578,18 @@ template <typename F>
 static auto with_attend(const KvPaged *kv, F use)
 {
     using namespace kvp;
-#define KVP_KERNEL(KV, HSP, BOXES) \
-    use(attend_kernel<KV, HSP, BOXES>, 32 * Geo<KV, HSP, BOXES>::WARPS, Geo<KV, HSP, BOXES>::SMEM, Geo<KV, HSP, BOXES>::PART, \
-        Geo<KV, HSP, BOXES>::TILE)
-#define KVP_CASE(KV, HSP) (kv->boxes ? KVP_KERNEL(KV, HSP, true) : KVP_KERNEL(KV, HSP, false))
-    if (kv->s.type == 1) return kv->hsp == 64 ? KVP_CASE(__half, 64) : kv->hsp == 128 ? KVP_CASE(__half, 128) : KVP_CASE(__half, 256);
-    return kv->hsp == 64 ? KVP_CASE(float, 64) : kv->hsp == 128 ? KVP_CASE(float, 128) : KVP_CASE(float, 256);
-#undef KVP_KERNEL
+#define KVP_KERNEL(KV, HSP, BOXES, PLAIN)                                                                      \
+    use(attend_kernel<KV, HSP, BOXES, PLAIN>, 32 * Geo<KV, HSP, BOXES, PLAIN>::WARPS, Geo<KV, HSP, BOXES, PLAIN>::SMEM, \
+        Geo<KV, HSP, BOXES, PLAIN>::PART, Geo<KV, HSP, BOXES, PLAIN>::TILE)
+#define KVP_CASE(KV, HSP, PLAIN) (kv->boxes ? KVP_KERNEL(KV, HSP, true, PLAIN) : KVP_KERNEL(KV, HSP, false, PLAIN))
+#define KVP_SIZES(KV, PLAIN) \
+    (kv->hsp == 64 ? KVP_CASE(KV, 64, PLAIN) : kv->hsp == 128 ? KVP_CASE(KV, 128, PLAIN) : KVP_CASE(KV, 256, PLAIN))
+    if (kv->s.type == 1) return KVP_SIZES(__half, 0);
+    const int group = kv->s.n_heads / kv->s.n_kv_heads;
+    return group == 1 ? KVP_SIZES(float, 1) : group == 2 ? KVP_SIZES(float, 2) : KVP_SIZES(float, 0);
+#undef KVP_SIZES
 #undef KVP_CASE
+#undef KVP_KERNEL
 }
 
 static bool off16(const void *p)
