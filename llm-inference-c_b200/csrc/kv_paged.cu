@@ -382,7 +382,10 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendArgs a)
 // least, operands through shared memory and accumulators through tensor
 // memory) would do four times the work for the same bytes: the warp-level
 // mma takes its operands straight from the registers that the softmax leaves
-// them in.
+// them in. PLAIN: one or two heads on a float KV head leave most of the 16
+// rows empty, and are multiplied by packed float products instead, the KV
+// head's entries read once for both (16 rows of 1030 tokens, 32 KV heads of
+// 128: 91 instead of 101 us; four heads would gain nothing, 102 and 103).
 //
 // All items' tokens, cut into chunks, are shared out evenly over all resident
 // CTAs, whatever the rows' lengths. A warp takes every WARPS-th tile of a
@@ -412,14 +415,15 @@ constexpr float ATT_JOIN = 0.2f;  // the cost of a part over that of a chunk
 template <typename KV, int HSP, bool BOXES, int PLAIN>
 struct Geo {
     static constexpr bool HALF = sizeof(KV) == 2;
-    static constexpr int TILE = HALF ? (HSP <= 128 ? 32 : 16) : (HSP == 64 ? 16 : 8);  // tokens
+    static constexpr int TILE = HALF ? (HSP <= 128 ? 32 : 16) : (HSP <= 128 ? 16 : 8);  // tokens
     static constexpr int WARPS = 4;
-    // 16 KB a warp: one tile of 128 half or 256 channels, two of the others.
-    // One of 32 tokens instead of two of 16 spreads what a tile costs beyond
-    // its products over more of them (40 rows of up to 4000 tokens, 24 heads
-    // on 2 KV heads of 80: 35 instead of 45 us; 64 rows of up to 8192 the
-    // same); twelve warps an SM cover the wait for the next.
-    static constexpr int STAGES = HSP == 256 || (HALF && HSP == 128) ? 1 : 2;
+    // 16 KB a warp: two tiles of 64 channels, or one. One of twice the tokens
+    // instead of two spreads what a tile costs beyond its products over more
+    // of them (half: 40 rows of up to 4000 tokens, 24 heads on 2 KV heads of
+    // 80, 35 instead of 45 us, 64 rows of up to 8192 the same; float: 16 rows
+    // of 2030, 32 heads on 16 KV heads, 89 instead of 93); twelve warps an SM
+    // cover the wait for the next.
+    static constexpr int STAGES = HSP >= 128 ? 1 : 2;
     static constexpr int CTAS = HSP == 256 ? 2 : 3;  // per SM, as shared memory allows
     static constexpr int CHUNK = WARPS * TILE;       // tokens: the unit in which work is shared out
     static constexpr int WIDE = HSP * (int)sizeof(KV) / 128;  // columns of 128 bytes
@@ -1146,21 +1150,27 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES, PLAIN>::WARPS, Geo<KV
                     for (int j = 0; j < NT; j++) rest[j][0] = rest[j][1] = rest[j][2] = rest[j][3] = 0.0f;
                     const uint32_t at = ks_s + (lane & 7) * 128, piece = ((lane >> 3) ^ (lane & 7)) << 4;
 #pragma unroll
-                    for (int ks = 0; ks < KS / 2; ks++) {
-                        uint32_t qa[4], qb[4];
-                        q_step(2 * ks, qa);
-                        q_step(2 * ks + 1, qb);
+                    for (int k2 = 0; k2 < KS / 4; k2++) {
+                        float z[NT][4];
 #pragma unroll
-                        for (int j = 0; j < NT; j++) {
-                            uint32_t kb[4];
-                            ldmatrix4(kb, at + k_eight[j] + (ks / 2) * column + (piece ^ ((ks & 1) << 6)));
-                            float z[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma_tf32(z, qa, kb[0], kb[1]);
-                            mma_tf32(rest[j], qa, rest_tf32(kb[0]), rest_tf32(kb[1]));
-                            mma_tf32(z, qb, kb[2], kb[3]);
-                            mma_tf32(rest[j], qb, rest_tf32(kb[2]), rest_tf32(kb[3]));
-                            add_tile(s[j], z, 1.0f);
+                        for (int j = 0; j < NT; j++) z[j][0] = z[j][1] = z[j][2] = z[j][3] = 0.0f;
+#pragma unroll
+                        for (int ks = 2 * k2; ks < 2 * k2 + 2; ks++) {
+                            uint32_t qa[4], qb[4];
+                            q_step(2 * ks, qa);
+                            q_step(2 * ks + 1, qb);
+#pragma unroll
+                            for (int j = 0; j < NT; j++) {
+                                uint32_t kb[4];
+                                ldmatrix4(kb, at + k_eight[j] + (ks / 2) * column + (piece ^ ((ks & 1) << 6)));
+                                mma_tf32(z[j], qa, kb[0], kb[1]);
+                                mma_tf32(rest[j], qa, rest_tf32(kb[0]), rest_tf32(kb[1]));
+                                mma_tf32(z[j], qb, kb[2], kb[3]);
+                                mma_tf32(rest[j], qb, rest_tf32(kb[2]), rest_tf32(kb[3]));
+                            }
                         }
+#pragma unroll
+                        for (int j = 0; j < NT; j++) add_tile(s[j], z[j], 1.0f);
                     }
 #pragma unroll
                     for (int j = 0; j < NT; j++) add_tile(s[j], rest[j], 1.0f);
