@@ -136,7 +136,8 @@ int kv_paged_append(KvPaged *kv, const float *q, const float *k, const float *v,
  * and its output left as it was. Entries of the pools behind a row's
  * position are never used, whatever they hold. A q or a visible entry that is
  * not finite (or 2^127 and more, in an F32 pool) makes the outputs that it
- * enters not finite, without regard to the signs of infinities. n is at
+ * enters not finite, without regard to the signs of infinities; only where a
+ * token's score is -infinity it may count as a token that is not there. n is at
  * most 65535; table has n_requests (<= max_requests) rows. q and out: rows of
  * n_heads * head_size floats on 16 bytes, q_stride as in kv_paged_append; out
  * must not overlap q. Results do not depend on timing: the same inputs give

@@ -1015,10 +1015,13 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES, PLAIN>::WARPS, Geo<KV
             uint32_t mask = 0u;
             if (BOXES) {
                 if (!lost && !arrived(bar_s + 8 * slot, (phases >> slot) & 1u)) {
-                    // nothing more is asked for, and what is left counts for nothing
+                    // nothing more is asked for, what is left counts for
+                    // nothing, and copies under way get their time to end
                     atomicOr(a.err, KV_PAGED_TIMEOUT);
                     lost = true;
                     l_more = nx_any = false;
+#pragma unroll 1
+                    for (int i = 0; i < G::STAGES; i++) arrived(bar_s + 8 * i, (phases >> i) & 1u);
                 }
                 phases ^= 1u << slot;
             } else {

@@ -409,6 +409,20 @@ def test_attend_never_uses_what_is_behind_a_row(torch, kind, value, hs, page):
     s.kv.close()
 
 
+@pytest.mark.parametrize("heads,kvh", [(3, 3), (6, 3)])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("hs,page", [(32, 8), (64, 16), (64, 7), (72, 32), (128, 8), (128, 64), (160, 40), (256, 5),
+                                     (256, 16)])
+def test_attend_few_heads_never_use_what_is_behind_a_row(torch, heads, kvh, value, hs, page):
+    s = Setup(torch, "f32", "token", heads, kvh, hs, page, [1, 5, 16, 18, 47, 100, 0, 130])
+    s.spoil(value)
+    out = s.run()
+    assert np.isfinite(out).all()
+    assert (out[6] == 0).all()
+    s.check(out)
+    s.kv.close()
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16"])
 def test_attend_rows_of_one_request_and_rows_passed_over(torch, kind):
     """Several rows of a request at different positions, in any order, rows
