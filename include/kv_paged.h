@@ -121,8 +121,9 @@ int kv_paged_map(KvPaged *kv, const int *len, const int *start, const int *end, 
  * q and q_out: rows of n_heads * head_size floats; q_out may be q, and q and
  * q_out may both be NULL. k and v: rows of n_kv_heads * head_size floats.
  * q_stride and kv_stride: floats from a row of q, and of k and v, to the
- * next (0: without gaps; multiples of 4). q_out has no gaps unless it is q.
- * All but row_pos and row_slot on 16 bytes (rope_cs on 8).
+ * next (0: without gaps; multiples of 4). q_out has no gaps unless it is q,
+ * and else does not overlap it. All but row_pos and row_slot on 16 bytes
+ * (rope_cs on 8).
  */
 int kv_paged_append(KvPaged *kv, const float *q, const float *k, const float *v, const int *row_pos,
                     const int *row_slot, int n, float *q_out, void *k_pool, void *v_pool, const float *rope_cs,

@@ -1610,6 +1610,13 @@ static bool off16(const void *p)
     return ((uintptr_t)p & 15) != 0;
 }
 
+// Whether any of these lists of 32-bit numbers is not on 4 bytes.
+template <typename... P>
+static bool off4(const P *...p)
+{
+    return (((uintptr_t)p | ...) & 3) != 0;
+}
+
 extern "C" KvPaged *kv_paged_open(const KvPagedShape *shape, int device, char *error, size_t cap)
 {
     auto fail = [&](const char *why) -> KvPaged * {
@@ -1727,6 +1734,8 @@ extern "C" int kv_paged_map(KvPaged *kv, const int *len, const int *start, const
     if (n < 1 || n > kv->s.max_requests) return refuse(kv, "map: requests outside 1 .. max_requests.");
     if (max_rows < 0 || max_rows > 1 << 30 || (max_rows > 0 && (!row_request || !row_pos || !row_slot)))
         return refuse(kv, "map: no room for the rows.");
+    if (off4(len, start, end, table, free_pages, n_free, n_free_out, row_request, row_pos, row_slot, row0))
+        return refuse(kv, "map: a pointer is not on 4 bytes.");
     if (kv->device < 0) return refuse(kv, "The handle has no device.");
     OnDevice on(kv->device);
     if (!on.ok) return refuse(kv, "CUDA device cannot be used.");
@@ -1769,6 +1778,11 @@ extern "C" int kv_paged_append(KvPaged *kv, const float *q, const float *k, cons
     if (off16(q) || off16(k) || off16(v) || off16(q_out) || off16(k_pool) || off16(v_pool) ||
         ((uintptr_t)rope_cs & 7))
         return refuse(kv, "append: a pointer is not on 16 bytes (the rotary table: 8).");
+    if (off4(row_pos, row_slot)) return refuse(kv, "append: a pointer is not on 4 bytes.");
+    const char *q0 = (const char *)q, *o0 = (const char *)q_out;
+    if (n > 0 && q != q_out && q0 < o0 + (size_t)n * qd * 4 && o0 < q0 + ((size_t)(n - 1) * q_stride + qd) * 4)
+        return refuse(kv, "append: q_out overlaps q and is not q.");
+    if (k_pool == v_pool) return refuse(kv, "append: keys and values have one pool.");
     if (kv->device < 0) return refuse(kv, "The handle has no device.");
     if (n == 0) return 1;
     OnDevice on(kv->device);
@@ -1807,6 +1821,7 @@ extern "C" int kv_paged_attend(KvPaged *kv, const float *q, const void *k_pool, 
     if (q_stride < qd || q_stride % 4) return refuse(kv, "attend: the row stride is too small or no multiple of 4.");
     if (off16(q) || off16(k_pool) || off16(v_pool) || off16(out))
         return refuse(kv, "attend: a pointer is not on 16 bytes.");
+    if (off4(table, row_request, row_pos)) return refuse(kv, "attend: a pointer is not on 4 bytes.");
     const char *q0 = (const char *)q, *o0 = (const char *)out;
     if (n > 0 && q0 < o0 + (size_t)n * qd * 4 && o0 < q0 + ((size_t)(n - 1) * q_stride + qd) * 4)
         return refuse(kv, "attend: out overlaps q.");
