@@ -1064,8 +1064,12 @@ int engine_forward_batch(LLMModel *m, const int *tokens, const int *pos, const i
             return 0;
         }
     }
-    if (!pkb_step(m->batch, tokens, pos, seq_ids, n, next_tokens, logits)) {
+    const int done = pkb_step(m->batch, tokens, pos, seq_ids, n, next_tokens, logits);
+    if (done != 1) {
         snprintf(m->last_error, sizeof(m->last_error), "%s", pkb_error(m->batch));
+        /* the rows of a paged step that had begun are there to be fed again */
+        for (int i = 0; done < 0 && m->batch_paged && i < n; i++)
+            if (m->filled[seq_ids[i]] > pos[i]) m->filled[seq_ids[i]] = pos[i];
         return 0;
     }
     for (int i = 0; m->batch_paged && i < n; i++) m->filled[seq_ids[i]] = 0;
@@ -1108,7 +1112,7 @@ int engine_prefill(LLMModel *m, const int *tokens, int n, int pos0, float *last_
                 return -2;
             }
         }
-        if (!pkb_step(m->prefill, tokens + i0, pos, seq, k, next, final ? lg : NULL)) {
+        if (pkb_step(m->prefill, tokens + i0, pos, seq, k, next, final ? lg : NULL) != 1) {
             snprintf(m->last_error, sizeof(m->last_error), "%s", pkb_error(m->prefill));
             seterr(err, cap, m->last_error);
             free(lg);

@@ -1426,19 +1426,22 @@ extern "C" int pkb_step(PkbCtx *b, const int *tokens, const int *pos, const int 
     }
     if (bfail(b, cudaGraphLaunch(b->exec[wl][n], b->st), "graph launch") ||
         bfail(b, cudaStreamSynchronize(b->st), "batched step"))
-        return 0;
+        return -1;
+    if (b->paged) {
+        // the pages are dealt out, unless the map was refused, whatever went wrong behind it
+        const int bits = b->io_h[4 * B + 1];
+        if (!(bits & (KV_PAGED_NO_PAGES | KV_PAGED_NO_ROWS | KV_PAGED_BAD_LENGTH)))
+            for (int s = 0; s < b->max_seqs; s++) b->len[s] = b->pg_h[2 * B + s];
+        if (bits != 0) {
+            snprintf(b->msg, sizeof(b->msg), "The paged cache reported an error (error word %d).", bits);
+            kv_paged_error(b->paged);  // clears it
+            return -1;
+        }
+    }
     if (b->io_h[4 * B] != 0) {
         snprintf(b->msg, sizeof(b->msg), "A device wait of the batched step ran out of time (error word %d).",
                  b->io_h[4 * B]);
-        return 0;
-    }
-    if (b->paged) {
-        for (int s = 0; s < b->max_seqs; s++) b->len[s] = b->pg_h[2 * B + s];
-        if (b->io_h[4 * B + 1] != 0) {
-            snprintf(b->msg, sizeof(b->msg), "The paged cache reported an error (error word %d).", b->io_h[4 * B + 1]);
-            kv_paged_error(b->paged);  // clears it
-            return 0;
-        }
+        return -1;
     }
     for (int i = 0; i < n; i++) next[order[i]] = b->io_h[3 * B + i];
     if (b->paged) {
@@ -1446,14 +1449,14 @@ extern "C" int pkb_step(PkbCtx *b, const int *tokens, const int *pos, const int 
         for (int i = 0; logits != NULL && i < n; i++)
             if (bfail(b, cudaMemcpyAsync(logits + order[i] * row, b->logits + i * row, row * 4, cudaMemcpyDeviceToHost, b->st),
                       "logits copy"))
-                return 0;
-        return logits == NULL || !bfail(b, cudaStreamSynchronize(b->st), "logits copy");
+                return -1;
+        return logits != NULL && bfail(b, cudaStreamSynchronize(b->st), "logits copy") ? -1 : 1;
     }
     if (logits != NULL &&
         bfail(b, cudaMemcpy(logits, wl ? b->logits_full : b->logits, (size_t)n * b->m.vocab_size * 4,
                             cudaMemcpyDeviceToHost),
               "logits copy"))
-        return 0;
+        return -1;
     return 1;
 }
 

@@ -162,7 +162,8 @@ void pkb_destroy(PkbCtx *b);
  * vocab floats, host) when not NULL. Arguments are checked by the caller; a
  * paged state's rows of one sequence are consecutive positions, and the
  * sequence ends with the last of them afterwards.
- * Returns 1, or 0 on a device error (message in pkb_error). */
+ * Returns 1, 0 when nothing was launched, -1 when the step had begun (message
+ * in pkb_error). */
 int pkb_step(PkbCtx *b, const int *tokens, const int *pos, const int *seq_ids, int n, int *next, float *logits);
 const char *pkb_error(const PkbCtx *b);
 
