@@ -100,9 +100,10 @@ __host__ __device__ __forceinline__ int pages_of(const Div &page, int x)
 // memory (lengths, pages, then the rows' stores): 64 requests take 3.0 us. Many
 // rows are bound by their 12 bytes each: a thread then finds the request of
 // ROWS = 4 rows with one search and stores them in 16 bytes (two million rows
-// of 256 requests 10 us, 2.5 TB/s; a row a thread 17 us). More than 1024
-// requests take CTAs of 1024 threads, since every CTA sums over all of them
-// (4096 requests 13 us, with 256 threads 27).
+// of 256 requests 10 us, 2.5 TB/s; a row a thread 17 us). More than 768
+// requests (1024 with many rows) take CTAs of 1024 threads, since every CTA
+// sums over all of them (1000 requests, 24000 rows: 6.1 us, with 256 threads
+// 7.4; 700: 6.0 and 5.4; 4096: 13 and 27).
 template <int THREADS, int ROWS>
 __global__ void __launch_bounds__(THREADS) map_kernel(const MapArgs a)
 {
@@ -1372,12 +1373,18 @@ __global__ void __launch_bounds__(32 * Geo<KV, HSP, BOXES, PLAIN>::WARPS, Geo<KV
     // ---- parts: the last of an item's CTAs to arrive joins them in their order ----
     __syncthreads();
     if (pend[0].parts == 0 && pend[1].parts == 0) return;
-    __threadfence();
-    __syncthreads();
+    // (the barrier above and this release order the parts' stores of all
+    // threads before the arrival, the acquire and the barrier below the others'
+    // parts before their loads)
     if (tid < 2) {
         const Part p = pend[tid];
-        is_last[tid] = p.parts > 0 && atomicInc(a.arrived + p.b0, (unsigned)p.parts - 1) == (unsigned)p.parts - 1;
-        __threadfence();
+        unsigned before_it = 0;
+        if (p.parts > 0)
+            asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
+                         : "=r"(before_it)
+                         : "l"(a.arrived + p.b0), "r"((unsigned)p.parts - 1)
+                         : "memory");
+        is_last[tid] = p.parts > 0 && before_it == (unsigned)p.parts - 1;
     }
     __syncthreads();
     for (int k = 0; k < 2; k++) {
@@ -1750,7 +1757,7 @@ extern "C" int kv_paged_map(KvPaged *kv, const int *len, const int *start, const
         kernel<<<(int)(ctas < 1 ? 1 : ctas < most ? ctas : most), threads, (6 * n + 3) * 4, (cudaStream_t)stream>>>(a);
     };
     const bool many = max_rows > kv->sms * 1024;
-    if (n > 1024) {
+    if (n > (many ? 1024 : 768)) {
         many ? go(kvp::map_kernel<1024, 4>, 1024, 4) : go(kvp::map_kernel<1024, 1>, 1024, 1);
     } else {
         many ? go(kvp::map_kernel<256, 4>, 256, 4) : go(kvp::map_kernel<256, 1>, 256, 1);
@@ -1782,7 +1789,6 @@ extern "C" int kv_paged_append(KvPaged *kv, const float *q, const float *k, cons
     const char *q0 = (const char *)q, *o0 = (const char *)q_out;
     if (n > 0 && q != q_out && q0 < o0 + (size_t)n * qd * 4 && o0 < q0 + ((size_t)(n - 1) * q_stride + qd) * 4)
         return refuse(kv, "append: q_out overlaps q and is not q.");
-    if (k_pool == v_pool) return refuse(kv, "append: keys and values have one pool.");
     if (kv->device < 0) return refuse(kv, "The handle has no device.");
     if (n == 0) return 1;
     OnDevice on(kv->device);

@@ -79,7 +79,7 @@ def call(kv, name, **change):
     a = dict(
         map=dict(len_ptr=P, start=P, end=P, n=4, table=P, free_pages=P, n_free=P, n_free_out=P, max_rows=9, row_request=P,
                  row_pos=P, row_slot=P, row0=P),
-        append=dict(q=P, k=P, v=P, row_pos=P, row_slot=P, n=3, q_out=P, k_pool=P, v_pool=2 * P, rope_cs=P, rope_dim=64,
+        append=dict(q=P, k=P, v=P, row_pos=P, row_slot=P, n=3, q_out=P, k_pool=P, v_pool=P, rope_cs=P, rope_dim=64,
                     rope_len=10),
         attend=dict(q=P, k_pool=P, v_pool=P, table=P, n_requests=4, row_request=P, row_pos=P, n=3, scale=0.1,
                     out=2 * P),
@@ -113,7 +113,6 @@ def call(kv, name, **change):
     *[("attend", {k: P + 2}, "4 bytes") for k in ("table", "row_request", "row_pos")],
     *[("append", dict(q_out=P + d), "overlaps") for d in (16, 2048, 3 * 2048 - 16, -16, 16 - 3 * 2048)],
     ("append", dict(q_stride=1024, q_out=P + 2 * 4096 + 2048 - 16), "overlaps"),
-    ("append", dict(v_pool=P), "one pool"),
 ])
 def test_calls_refused(name, change, why):
     kv = handle()
